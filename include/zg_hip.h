@@ -536,6 +536,163 @@ int zg_act_prepare_device(zg_ctx* ctx, const zg_weight* w, const void* x, int x_
 int zg_gemv_prepared_device(zg_ctx* ctx, const zg_weight* w, size_t m_rows, const void* prepared, float* y,
                             void* stream);
 
+/* ------------------------------------- paged KV cache and logits readout */
+
+/* A KV cache in pages on the device, the resident counterpart of the
+ * reference's paged block tables (core/src/paged_state.rs:239-330).  Element
+ * d of head h of slot s of page p is at p * page_stride + (s * kv_heads + h)
+ * * head_dim + d of keys and of values, in elements of dtype: a page is a
+ * piece of the token-major cache that zg_attn_decode_device takes, and keys
+ * and values may be interleaved in one pool.  head_dim 64, 128 or 256; dtype
+ * ZG_BF16 or ZG_F32; page_tokens 1..65536; page_stride a multiple of 64, at
+ * least page_tokens * kv_heads * head_dim; both pointers 16-byte aligned. */
+typedef struct zg_paged_kv {
+    void* keys;
+    void* values;
+    size_t pages, page_tokens, page_stride, kv_heads, head_dim;
+    int dtype;
+} zg_paged_kv;
+
+/* The page tables of a batch's rows: entry [r][i] of pages (device, row
+ * stride `stride` entries) is the page of row r's own tokens i * page_tokens
+ * and on.  Before its own tokens every row has the same prefix_tokens tokens,
+ * held in the pages that `prefix` lists (device; NULL when prefix_tokens is
+ * 0); the prefix may end inside a page.  Entries past a row's last token are
+ * never read and may hold anything. */
+typedef struct zg_paged_rows {
+    const int32_t* pages;
+    size_t rows, stride;
+    const int32_t* prefix;
+    size_t prefix_tokens;
+} zg_paged_rows;
+
+/* What the device found wrong, or-ed into the status word (device, int32)
+ * that a caller hands to the calls below; NULL when it does not ask.  The
+ * word is never cleared by a call. */
+enum { ZG_STATUS_PAGE = 1, ZG_STATUS_POSITION = 2, ZG_STATUS_NONFINITE = 4 };
+
+/* Host-only check of a cache, of `lengths` (host, [rows->rows], own tokens
+ * per row, negative: row not in use) and of page tables held in host memory
+ * (rows->pages, rows->prefix), as a scheduler makes it before it uploads them:
+ * ZG_E_MALFORMED for a page outside the pool or a length past the row's
+ * table, and the refusals of zg_paged_attn_device for the rest, with the
+ * reason in msg (msg_len bytes, NUL-terminated; may be NULL).  No context and
+ * no device; the pool's pointers are not followed. */
+int zg_paged_admit(const zg_paged_kv* cache, const zg_paged_rows* rows, const int32_t* lengths, size_t q_heads,
+                   char* msg, size_t msg_len);
+
+/* Append `tokens` tokens to a paged cache on the caller's stream (a prompt's
+ * chunk or one token per row), rotating positions on the way: query and key
+ * heads are RMS-normalised (lib.rs:289-306; q_norm, k_norm [head_dim], NULL:
+ * not), their first `rotate` elements turned in pairs (i, i + rotate/2) by
+ * the angle position * theta_scale^i (the pairing of source_rope_kv,
+ * lib.rs:1552-1577; the angle is formed in 64 bits and its sine and cosine in
+ * 32, where the reference multiplies it up in 32, so the two part by some
+ * 1e-6 of the angle), key and value rounded to the cache's type and stored in
+ * the slot of their position, the query written to q_out.  Replaces the
+ * RopeKvRegion (accelerator.rs:205-296) and the cache append for a resident
+ * paged cache.  q [tokens] of row stride q_stride with heads q_head_stride
+ * apart (the [q | gate] projection's 2 * head_dim, or head_dim); k, v
+ * [tokens][kv_heads * head_dim] of row strides k_stride, v_stride; all of
+ * dtype ZG_F32 or ZG_BF16, strides in elements and multiples of 4, pointers
+ * aligned to 4 elements.  q_heads 0 with q and q_out NULL appends only.  q_out
+ * [tokens][q_heads * head_dim] of dtype, contiguous; it may be q itself where
+ * q is contiguous.  positions [tokens] (device) counts from the prefix's
+ * first token, so a row's first own token is at rows->prefix_tokens;
+ * negative: the token is skipped, nothing of it is read or written.
+ * token_rows [tokens] (device) is each token's row, NULL: token t belongs to
+ * row t.  rotate 0 to head_dim, a multiple of 8.  The positions of one row in
+ * one call differ from each other; which of two tokens at one place stays is
+ * not defined.  A row or position outside the table (ZG_STATUS_POSITION) or a
+ * page outside the pool (ZG_STATUS_PAGE) stores no key and value; the query is
+ * written all the same.  To write the prefix itself, give its pages as a row
+ * with prefix_tokens 0.  Asynchronous. */
+int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_rows* rows, size_t tokens,
+                           size_t q_heads, const void* q, size_t q_stride, size_t q_head_stride, const void* k,
+                           size_t k_stride, const void* v, size_t v_stride, int dtype, const float* q_norm,
+                           const float* k_norm, float eps, size_t rotate, float theta_scale, const int32_t* positions,
+                           const int32_t* token_rows, void* q_out, int32_t* status, void* stream);
+
+/* Attention of one query token per row over the shared prefix and the row's
+ * own lengths[r] tokens (device, [rows->rows]), on the caller's stream; the
+ * prefix's keys and values are read once for the whole batch.  out[r][h] =
+ * sum_t e^(scale q.k_t - m) v_t / sum_t e^(scale q.k_t - m) with kv head h /
+ * (q_heads / kv_heads), the softmax of lib.rs:1352-1387 and the value sum of
+ * lib.rs:1276-1305 regrouped: sums in 32 bits; 32-bit queries enter the
+ * matrix products as three bfloat16 parts (24 bits in all).  No counterpart in
+ * the reference, whose cohorts read each row's cache by itself.  q
+ * [rows][q_heads * head_dim] of row stride q_stride and out of row stride
+ * out_stride, both of dtype ZG_F32 or ZG_BF16, 16-byte aligned, strides
+ * multiples of 8; out may be q.  q_heads a multiple of kv_heads, at most 16
+ * times it; at most 4096 rows; rows->stride * page_tokens and prefix_tokens
+ * at most 2^30.  Several tokens of one sequence are rows with the same pages
+ * and their own lengths.  A row without any token (length 0, no prefix) gives
+ * zeros; a negative length leaves the row's out as it was.  A length past the
+ * row's table is cut to it (ZG_STATUS_POSITION); tokens of a page outside the
+ * pool are left out (ZG_STATUS_PAGE).  What slots past a row's length hold
+ * does not matter.  workspace of zg_paged_attn_workspace_bytes bytes (0 for
+ * arguments that the call refuses), 16-byte aligned, is written and read by
+ * the call: calls, and replays of captured ones, that may run at the same
+ * time need one each.  A captured call keeps prefix_tokens and the pointers,
+ * and reads the tables and lengths anew at each replay.  Asynchronous. */
+size_t zg_paged_attn_workspace_bytes(const zg_paged_kv* cache, const zg_paged_rows* rows, size_t q_heads);
+int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_rows* rows, const int32_t* lengths,
+                         size_t q_heads, const void* q, size_t q_stride, int dtype, float scale, void* workspace,
+                         void* out, size_t out_stride, int32_t* status, void* stream);
+
+/* What is done to a batch's logits before the readout; device pointers, NULL:
+ * that rule is off.  history [rows][history_stride] holds each row's tokens,
+ * prompt first, history_lengths[r] of them (a negative length: the row is
+ * left out of the call, its logits and id as they were), the first
+ * prompt_lengths[r] (NULL: none) the prompt.  Ids outside the vocabulary
+ * count for nothing.  Per row: repetition r > 0 divides a positive and
+ * multiplies any other logit of a token in the history; frequency f and
+ * presence p take f * count + p from a token generated `count` > 0 times
+ * (after the prompt).  bias_ids, bias_values [rows][bias_stride],
+ * bias_lengths[r] of them: added to their tokens' logits, an id that is there
+ * twice with the sum.  masks [mask_rows][mask_stride]: bit t % 32 of word t /
+ * 32 set allows token t; row r takes mask mask_of[r] (NULL: r), negative: any
+ * token is allowed.  A forbidden token's logit becomes -inf, whatever it
+ * was.  A rule's arrays are all there or all NULL: the history with its
+ * lengths, the biases' three. */
+typedef struct zg_logit_rules {
+    int32_t* history;
+    size_t history_stride;
+    int32_t* history_lengths;
+    const int32_t* prompt_lengths;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int32_t* bias_ids;
+    const float* bias_values;
+    size_t bias_stride;
+    const int32_t* bias_lengths;
+    const uint32_t* masks;
+    size_t mask_rows, mask_stride;
+    const int32_t* mask_of;
+} zg_logit_rules;
+
+/* Apply the rules to logits [rows][vocab] (row stride ld) of dtype ZG_F32 or
+ * ZG_BF16 on the caller's stream and write them to out (row stride out_ld; it
+ * may be logits itself, with the same stride): repetition, then frequency
+ * and presence, then biases, in 64 bits and rounded once, then the mask.  The
+ * readout of zg_greedy over what may be masked: greedy[r] (device, NULL: not
+ * asked) is the index of the highest of the row's values as written, the
+ * lowest index of equal ones; NaN and -inf are never taken, and 0xffffffff
+ * stands where nothing is left.  A NaN or +inf among the allowed tokens raises
+ * ZG_STATUS_NONFINITE.  record 1 also stores a row's greedy id behind its
+ * history and counts history_lengths[r] up, while history_stride has room;
+ * it needs a history and greedy.  No counterpart in the reference, whose
+ * readout is greedy_finite alone (core/src/numerics.rs:124-140).  At most
+ * 65535 rows and a vocabulary of 2^30; at most 65535 biases a row.  workspace
+ * of zg_logits_adjust_workspace_bytes bytes, 16-byte aligned, needed with
+ * greedy (else NULL), one for each call that may run at the same time.
+ * Asynchronous. */
+size_t zg_logits_adjust_workspace_bytes(size_t rows, size_t vocab);
+int zg_logits_adjust_device(zg_ctx* ctx, size_t rows, size_t vocab, const void* logits, size_t ld, int dtype,
+                            const zg_logit_rules* rules, void* out, size_t out_ld, uint32_t* greedy, int record,
+                            void* workspace, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

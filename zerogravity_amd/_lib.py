@@ -20,6 +20,27 @@ P = C.c_void_p
 SZ = C.c_size_t
 FP = C.POINTER(C.c_float)
 
+
+class PagedKv(C.Structure):
+    """zg_paged_kv"""
+    _fields_ = [("keys", P), ("values", P), ("pages", SZ), ("page_tokens", SZ), ("page_stride", SZ), ("kv_heads", SZ),
+                ("head_dim", SZ), ("dtype", C.c_int)]
+
+
+class PagedRows(C.Structure):
+    """zg_paged_rows"""
+    _fields_ = [("pages", P), ("rows", SZ), ("stride", SZ), ("prefix", P), ("prefix_tokens", SZ)]
+
+
+class LogitRules(C.Structure):
+    """zg_logit_rules"""
+    _fields_ = [("history", P), ("history_stride", SZ), ("history_lengths", P), ("prompt_lengths", P),
+                ("repetition", P), ("frequency", P), ("presence", P), ("bias_ids", P), ("bias_values", P),
+                ("bias_stride", SZ), ("bias_lengths", P), ("masks", P), ("mask_rows", SZ), ("mask_stride", SZ),
+                ("mask_of", P)]
+
+
+
 _SIGS = {
     "zg_version": (C.c_char_p, []),
     "zg_ctx_create": (C.c_int, [C.c_int, C.POINTER(P)]),
@@ -88,6 +109,15 @@ _SIGS = {
     "zg_snapshot_bytes": (SZ, [P]),
     "zg_snapshot_position": (C.c_int, [P]),
     "zg_snapshot_destroy": (None, [P]),
+    "zg_paged_admit": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), P, SZ, C.c_char_p, SZ]),
+    "zg_paged_append_device": (C.c_int, [P, C.POINTER(PagedKv), C.POINTER(PagedRows), SZ, SZ, P, SZ, SZ, P, SZ, P, SZ,
+                                         C.c_int, P, P, C.c_float, SZ, C.c_float, P, P, P, P, P]),
+    "zg_paged_attn_workspace_bytes": (SZ, [C.POINTER(PagedKv), C.POINTER(PagedRows), SZ]),
+    "zg_paged_attn_device": (C.c_int, [P, C.POINTER(PagedKv), C.POINTER(PagedRows), P, SZ, P, SZ, C.c_int, C.c_float,
+                                       P, P, SZ, P, P]),
+    "zg_logits_adjust_workspace_bytes": (SZ, [SZ, SZ]),
+    "zg_logits_adjust_device": (C.c_int, [P, SZ, SZ, P, SZ, C.c_int, C.POINTER(LogitRules), P, SZ, P, C.c_int, P, P,
+                                          P]),
 }
 
 
@@ -134,6 +164,7 @@ class Context:
         if rc != COMPLETED:
             raise ZgError(rc, "zg_ctx_create failed (no usable HIP device?)")
         self.h = h
+        self.device = device
         self._dependents = []  # weakrefs to models/sessions living on this ctx
 
     def adopt(self, obj):
