@@ -625,7 +625,8 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
  * out_stride, both of dtype ZG_F32 or ZG_BF16, 16-byte aligned, strides
  * multiples of 8; out may be q.  q_heads a multiple of kv_heads, at most 16
  * times it; at most 4096 rows; rows->stride * page_tokens and prefix_tokens
- * at most 2^30.  Several tokens of one sequence are rows with the same pages
+ * at most 2^30, rows * kv_heads * stride * page_tokens below
+ * 2^35.  Several tokens of one sequence are rows with the same pages
  * and their own lengths.  A row without any token (length 0, no prefix) gives
  * zeros; a negative length leaves the row's out as it was.  A length past the
  * row's table is cut to it (ZG_STATUS_POSITION); tokens of a page outside the

@@ -90,7 +90,8 @@ struct LogitArgs {
 
 hipError_t paged_append(const AppendArgs& a, hipStream_t st);
 hipError_t paged_attn(const PagedAttnArgs& a, hipStream_t st);
-size_t paged_attn_workspace(uint32_t rows, int q_heads, int kv_heads, int head_dim, uint32_t prefix_tokens);
+size_t paged_attn_workspace(uint32_t rows, int q_heads, int kv_heads, int head_dim, int bf16, uint32_t prefix_tokens,
+                            uint64_t row_tokens);
 hipError_t logits_adjust(const LogitArgs& a, hipStream_t st);
 size_t logits_workspace(size_t rows, size_t vocab);
 

@@ -70,6 +70,9 @@ Refusal check_attention(const zg_paged_kv* c, const zg_paged_rows* r, size_t q_h
     if (Refusal why = check_rows(c, r)) return why;
     if (r->prefix_tokens && !r->prefix) return {ZG_E_MALFORMED, "a prefix without its pages"};
     if (q_heads == 0 || q_heads % c->kv_heads) return {ZG_E_MALFORMED, "query heads are a multiple of the kv heads"};
+    // the rows' tiles of 16 or 32 tokens are counted in 32 bits
+    if ((r->stride * c->page_tokens + 15) / 16 >= ((size_t)1 << 31) / (r->rows * c->kv_heads))
+        return {ZG_E_LIMIT, "rows * kv_heads * tokens a row can hold is at most 2^35"};
     if (q_heads / c->kv_heads > 16) return {ZG_E_UNSUPPORTED, "at most 16 query heads to a kv head"};
     return {};
 }
@@ -210,8 +213,8 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
 
 size_t zg_paged_attn_workspace_bytes(const zg_paged_kv* cache, const zg_paged_rows* rows, size_t q_heads) {
     if (check_attention(cache, rows, q_heads)) return 0;
-    return zg::paged_attn_workspace((uint32_t)rows->rows, (int)q_heads, (int)cache->kv_heads, (int)cache->head_dim,
-                                    (uint32_t)rows->prefix_tokens);
+    return zg::paged_attn_workspace((uint32_t)rows->rows, (int)q_heads, (int)cache->kv_heads, (int)cache->head_dim, cache->dtype == ZG_BF16,
+                                    (uint32_t)rows->prefix_tokens, (uint64_t)rows->stride * cache->page_tokens);
 }
 
 int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_rows* rows, const int32_t* lengths,
