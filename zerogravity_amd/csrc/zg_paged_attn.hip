@@ -28,8 +28,10 @@ namespace zg {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
-constexpr int kOwnGroups = 256;     // workgroups over the rows' own tiles
+constexpr int kOwnWaves = 2048;     // waves over the rows' own tiles: two per SIMD
+constexpr int kManyTiles = 2;       // fewest tiles of a piece of the prefix for 128 queries
 constexpr int kPrefixGroups = 256;  // about so many over the prefix
+constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
 constexpr float kRaise = 8.0f;      // log2: how far a score may pass the reference before sums are rescaled
 
 template <bool IO, bool KV, int D>
@@ -59,7 +61,7 @@ __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// Queries in LDS in operand order, 16 bytes per (part, step, quarter, query):
+// Queries in LDS in operand order, 16 bytes per (step, part, quarter, query):
 // a wave's read is contiguous.  `who` gives query m's elements in memory.
 template <bool IO, bool KV, int D, typename Who>
 __device__ __forceinline__ void stage_queries(v4u* lds, int n, int thread, int threads, Who who) {
@@ -79,7 +81,7 @@ __device__ __forceinline__ void stage_queries(v4u* lds, int n, int thread, int t
                 v4u w;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = pack_high(x[j >> 1][(2 * j) & 3], x[j >> 1][(2 * j + 1) & 3]);
-                lds[(p * (D / E) + c) * n + m] = w;
+                lds[((c / 4 * F::kParts + p) * 4 + (c & 3)) * n + m] = w;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j >> 2][j & 3] -= high_part(x[j >> 2][j & 3]);
             }
@@ -104,22 +106,116 @@ struct Sums {
     }
 };
 
-// Where a tile's tokens lie: every lane finds token lane % TILE, and a ballot
-// says which are there.
+// Where a tile's tokens lie: every lane takes token lane % TILE.  peek asks
+// the table, a tile ahead of its use; resolve makes a place of the answer,
+// and a ballot over ok says which tokens are there.
 struct Place {
     uint32_t unit;
     bool ok, stray;
 };
 template <int TILE>
-__device__ __forceinline__ Place find(const PagedPool& p, const int32_t* table, uint32_t tokens, int tile, int lane) {
+__device__ __forceinline__ uint32_t peek(const PagedPool& p, const int32_t* table, uint32_t tokens, int tile, int lane) {
+    return (uint32_t)table[p.page_tokens.quotient(min((uint32_t)tile * TILE + (lane & (TILE - 1)), tokens - 1))];
+}
+template <int TILE>
+__device__ __forceinline__ Place resolve(const PagedPool& p, uint32_t page, uint32_t tokens, int tile, int lane) {
     const uint32_t t = (uint32_t)tile * TILE + (lane & (TILE - 1));
-    const uint32_t pg = p.page_tokens.quotient(min(t, tokens - 1));
-    const uint32_t page = (uint32_t)table[pg];
     Place at;
     at.stray = page >= p.pages;
     at.ok = t < tokens && !at.stray;
-    at.unit = at.ok ? page * p.page_units + (t - pg * p.page_tokens.d) * p.slot_units : 0;
+    at.unit = at.ok ? page * p.page_units + (t - p.page_tokens.quotient(t) * p.page_tokens.d) * p.slot_units : 0;
     return at;
+}
+
+// A tile's weights e^(s - m) from its scores, m the query's reference: the
+// sums are brought to a new one only when a score passes the old one by
+// 2^kRaise, which 32-bit sums hold with ease.
+template <bool IO, bool KV, int D, int MT>
+__device__ __forceinline__ void weigh(const v4f (&sc)[MT][Form<IO, KV, D>::kHalves], uint32_t there, float to_log2,
+                                      int quarter, Sums<D, MT>& s, float (&w)[MT][Form<IO, KV, D>::kMine]) {
+    constexpr int N = Form<IO, KV, D>::kMine;
+    constexpr uint32_t kAll = N == 8 ? 0xffffffffu : 0xffffu;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            w[m][j] = sc[m][j >> 2][j & 3] * to_log2;
+            if (there != kAll && !(there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u)) w[m][j] = -INFINITY;
+            top = fmaxf(top, w[m][j]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        if (__any(top > s.ref[m] + kRaise)) {
+            const float to = fmaxf(top, s.ref[m]);
+            const float keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.ref[m] - to);
+            s.ref[m] = to;
+            s.l[m] *= keep;
+#pragma unroll
+            for (int f = 0; f < D / 16; ++f) s.o[m][f] *= keep;
+        }
+        const float sub = s.ref[m] == -INFINITY ? 0.0f : s.ref[m];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            w[m][j] = __builtin_amdgcn_exp2f(w[m][j] - sub);
+            s.l[m] += w[m][j];
+        }
+    }
+}
+
+// Values of tokens that are not there weigh 0, and may be anything.
+template <bool KV, int N, int VR>
+__device__ __forceinline__ void drop_values(uint32_t (&v)[N][VR], uint32_t there, int quarter) {
+    if (there == (N == 8 ? 0xffffffffu : 0xffffu)) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t keep = (there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u) ? 0xffffffffu : 0u;
+#pragma unroll
+        for (int x = 0; x < VR; ++x) v[j][x] &= keep;
+    }
+}
+
+// One load's worth of a tile's value rows, weighted, added to the sums.
+template <bool IO, bool KV, int D, int MT, int N, int VR>
+__device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const float (&w)[MT][N], int g, Sums<D, MT>& s) {
+    using F = Form<IO, KV, D>;
+    constexpr int W = F::kWide;
+    if constexpr (KV) {
+        v4u part[MT][F::kWeightParts];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = w[m][j];
+#pragma unroll
+            for (int p = 0; p < F::kWeightParts; ++p) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[m][p][j] = pack_high(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] -= high_part(x[j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            v4u rows;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                rows[j] = __builtin_amdgcn_perm(v[2 * j + 1][i >> 1], v[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int p = 0; p < F::kWeightParts; ++p)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) s.o[m][g * W + i] = mfma_bf16(rows, part[m][p], s.o[m][g * W + i]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    s.o[m][g * W + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][i]), w[m][j],
+                                                                             s.o[m][g * W + i], 0, 0, 0);
+    }
 }
 
 // Tiles tile, tile + step, ... before `end` of one table added to the sums.
@@ -136,8 +232,9 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
     const char* const values = (const char*)a.pool.values;
     constexpr uint32_t kAll = H == 2 ? 0xffffffffu : 0xffffu;
     if (tile >= end) return;
-    Place at = find<F::kTile>(a.pool, table, tokens, tile, lane);
+    uint32_t page = peek<F::kTile>(a.pool, table, tokens, tile, lane);
     for (; tile < end; tile += step) {
+        const Place at = resolve<F::kTile>(a.pool, page, tokens, tile, lane);
         if (at.stray) bad |= ZG_STATUS_PAGE;
         const uint32_t there = (uint32_t)__ballot(at.ok) & kAll;
         v4u k[H][F::kSteps];
@@ -148,25 +245,32 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
 #pragma unroll
             for (int i = 0; i < F::kSteps; ++i) k[h][i] = *(const v4u*)(row + 64 * i);
         }
-        uint32_t v[N][F::kLoads][VR];
+        // values: half of them now, half into the keys' registers once those
+        // are used up, so that a lane needs at most 256
+        uint32_t v[F::kLoads][N][VR];
+        const char* vrow[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const char* row = values + ((uint64_t)(uint32_t)__shfl((int)at.unit, 16 * (j >> 2) + 4 * quarter + (j & 3)) * 64 +
-                                        (uint32_t)kvh * D + W * col) * ES;
+        for (int j = 0; j < N; ++j)
+            vrow[j] = values + ((uint64_t)(uint32_t)__shfl((int)at.unit, 16 * (j >> 2) + 4 * quarter + (j & 3)) * 64 +
+                                (uint32_t)kvh * D + W * col) * ES;
+        auto load_values = [&](int g) {
 #pragma unroll
-            for (int g = 0; g < F::kLoads; ++g) {
+            for (int j = 0; j < N; ++j) {
                 if constexpr (VR == 4) {
-                    const v4u w = *(const v4u*)(row + 16 * W * g * ES);
+                    const v4u w = *(const v4u*)(vrow[j] + 16 * W * g * ES);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) v[j][g][x] = w[x];
+                    for (int x = 0; x < 4; ++x) v[g][j][x] = w[x];
                 } else {
-                    const uint2 w = *(const uint2*)(row + 16 * W * g * ES);
-                    v[j][g][0] = w.x;
-                    v[j][g][1] = w.y;
+                    const uint2 w = *(const uint2*)(vrow[j] + 16 * W * g * ES);
+                    v[g][j][0] = w.x;
+                    v[g][j][1] = w.y;
                 }
             }
-        }
-        if (tile + step < end) at = find<F::kTile>(a.pool, table, tokens, tile + step, lane);
+        };
+        constexpr int kFirst = (F::kLoads + 1) / 2;
+#pragma unroll
+        for (int g = 0; g < kFirst; ++g) load_values(g);
+        page = peek<F::kTile>(a.pool, table, tokens, tile + step, lane);
         __builtin_amdgcn_sched_barrier(0);
         // scores
         v4f sc[MT][H];
@@ -174,14 +278,17 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < H; ++h) sc[m][h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        // the queries' places are stepped through: kept for all steps they
+        // would take the registers of a quarter of the keys
+        int place = quarter * n + (MT == 1 ? min(col, n - 1) : col);
+        asm volatile("" : "+v"(place));
 #pragma unroll
         for (int i = 0; i < F::kSteps; ++i) {
 #pragma unroll
-            for (int p = 0; p < F::kParts; ++p)
+            for (int p = 0; p < F::kParts; ++p, place += 4 * n)
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const int q = MT == 1 ? min(col, n - 1) : 16 * m + col;
-                    const v4u b = queries[((p * F::kSteps + i) * 4 + quarter) * n + q];
+                    const v4u b = queries[place + 16 * m];
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
                         if constexpr (KV) {
@@ -197,82 +304,16 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
             // two steps' queries in registers at a time
             if (i & 1) __builtin_amdgcn_sched_barrier(0);
         }
-        // weights
-        float w[MT][N];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                w[m][j] = sc[m][j >> 2][j & 3] * to_log2;
-                if (there != kAll && !(there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u)) w[m][j] = -INFINITY;
-                top = fmaxf(top, w[m][j]);
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            if (__any(top > s.ref[m] + kRaise)) {
-                const float to = fmaxf(top, s.ref[m]);
-                const float keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.ref[m] - to);
-                s.ref[m] = to;
-                s.l[m] *= keep;
-#pragma unroll
-                for (int f = 0; f < F::kFrags; ++f) s.o[m][f] *= keep;
-            }
-            const float sub = s.ref[m] == -INFINITY ? 0.0f : s.ref[m];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                w[m][j] = __builtin_amdgcn_exp2f(w[m][j] - sub);
-                s.l[m] += w[m][j];
-            }
-        }
-        // values of tokens that are not there weigh 0, and may be anything
-        if (there != kAll) {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (!(there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u))
-#pragma unroll
-                    for (int g = 0; g < F::kLoads; ++g)
-#pragma unroll
-                        for (int x = 0; x < VR; ++x) v[j][g][x] = 0;
-        }
+        for (int g = kFirst; g < F::kLoads; ++g) load_values(g);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (KV) {
-            v4u part[MT][F::kWeightParts];
+        float w[MT][N];
+        weigh<IO, KV, D, MT>(sc, there, to_log2, quarter, s, w);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int p = 0; p < F::kWeightParts; ++p) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) part[m][p][j] = pack_high(w[m][2 * j], w[m][2 * j + 1]);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[m][j] -= high_part(w[m][j]);
-                }
-#pragma unroll
-            for (int g = 0; g < F::kLoads; ++g)
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    v4u rows;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        rows[j] = __builtin_amdgcn_perm(v[2 * j + 1][g][i >> 1], v[2 * j][g][i >> 1],
-                                                        i & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                    for (int p = 0; p < F::kWeightParts; ++p)
-#pragma unroll
-                        for (int m = 0; m < MT; ++m)
-                            s.o[m][g * W + i] = mfma_bf16(rows, part[m][p], s.o[m][g * W + i]);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-#pragma unroll
-                for (int g = 0; g < F::kLoads; ++g)
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-#pragma unroll
-                        for (int m = 0; m < MT; ++m)
-                            s.o[m][g * W + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                __uint_as_float(v[j][g][i]), w[m][j], s.o[m][g * W + i], 0, 0, 0);
+        for (int g = 0; g < F::kLoads; ++g) {
+            drop_values<KV>(v[g], there, quarter);
+            add_values<IO, KV, D, MT>(v[g], w, g, s);
         }
     }
 }
@@ -293,13 +334,14 @@ __device__ __forceinline__ void store_sums(float2* stats, float* o, size_t at, c
 }
 
 // How a call is cut.  The prefix: `chunks` pieces of chunk_tiles tiles, each
-// for `blocks` blocks of 16 MT queries and every kv head.  The rows' own
+// for `blocks` blocks of `block` queries and every kv head.  The rows' own
 // tiles, in the order (row, kv head, tile): wave w of the `waves` takes c
 // successive ones, c = ceil(all / waves), whatever rows they belong to, so
 // that long and short rows fill the card alike; where a wave's run crosses
 // from one (row, kv head) to the next it leaves one triple for each.
 struct Cut {
-    int prefix_tiles, chunk_tiles, chunks, blocks, waves;
+    int prefix_tiles, chunk_tiles, chunks, block, blocks, waves, per_group;  // per_group of the waves in a workgroup
+    uint2* runs;  // per (row, kv head): its first wave and how many hold a piece of it
     float2 *prefix_stats, *own_stats;
     float *prefix_o, *own_o;
 };
@@ -308,16 +350,34 @@ __device__ __forceinline__ uint32_t own_tokens(const PagedAttnArgs& a, uint32_t 
     const int n = a.lengths[r];
     return n < 0 ? 0 : min((uint32_t)n, a.stride * a.pool.page_tokens.d);
 }
-template <int TILE>
-__device__ __forceinline__ uint32_t own_tiles(const PagedAttnArgs& a, uint32_t r) {
-    return (own_tokens(a, r) + TILE - 1) / TILE;
+// The piece of the prefix that a workgroup takes.  Workgroups id, id + 8, id +
+// 16, ... run on one XCD: they are given the blocks of one piece, which that
+// L2 then reads from memory once.
+struct PieceOf {
+    int block, kvh, chunk;
+};
+__device__ __forceinline__ PieceOf piece_of(const Cut& c, int kv_heads, int id) {
+    const int pieces = c.chunks * kv_heads, whole = pieces / 8 * 8 * c.blocks;
+    PieceOf p;
+    int piece;
+    if (id < whole) {
+        p.block = id / 8 % c.blocks;
+        piece = id / (8 * c.blocks) * 8 + id % 8;
+    } else {
+        p.block = (id - whole) % c.blocks;
+        piece = (id - whole) / c.blocks + pieces / 8 * 8;
+    }
+    p.kvh = piece % kv_heads;
+    p.chunk = piece / kv_heads;
+    return p;
 }
 
 template <bool IO, bool KV, int D, int MT>
 __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
     using F = Form<IO, KV, D>;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
-    const int block = id % c.blocks, kvh = id / c.blocks % a.pool.kv_heads, chunk = id / c.blocks / a.pool.kv_heads;
+    const PieceOf at_piece = piece_of(c, a.pool.kv_heads, id);
+    const int block = at_piece.block, kvh = at_piece.kvh, chunk = at_piece.chunk;
     const int queries = (int)a.rows * a.group;
     struct {
         const void* base;
@@ -393,46 +453,81 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
             store_sums<F::kWide, D>(c.prefix_stats, c.prefix_o, at + 16 * m + col, s.o[m], ref[m], l[m], quarter);
 }
 
-template <bool IO, bool KV, int D>
+// What a wave wrote to LDS, its other lanes read after this.
+__device__ __forceinline__ void same_wave() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// LDS of own_block's table: 68 words for each wave, or one for all of them.
+__host__ __device__ inline size_t table_bytes(uint32_t rows, int waves) {
+    return rows <= 64 ? (size_t)waves * 68 * 4 : ((size_t)(rows + 1 + waves) * 4 + 15) / 16 * 16;
+}
+
+template <bool IO, bool KV, int D, int WAVES>
 __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
     using F = Form<IO, KV, D>;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
-    const int groups = c.waves / 4;
-    // tiles before each row, in LDS: thread t sums rows [t * per, (t + 1) * per)
-    uint32_t* ahead = (uint32_t*)lds;
-    uint32_t* sums = ahead + a.rows + 1;
-    const uint32_t per = (a.rows + 255) / 256;
-    uint32_t mine = 0;
+    const int groups = c.waves / c.per_group;
+    // ahead[r]: tiles of the rows before r, in LDS.  Up to 64 rows every wave
+    // finds them for itself, a row a lane, without a barrier; beyond, thread t
+    // sums rows [t * per, (t + 1) * per).
+    uint32_t* ahead = (uint32_t*)lds + (a.rows <= 64 ? wave * 68 : 0);
     int bad = 0;
-    for (uint32_t r = tid * per; r < min((tid + 1) * per, a.rows); ++r) {
-        mine += own_tiles<F::kTile>(a, r);
-        if ((int)a.lengths[r] > 0 && (uint32_t)a.lengths[r] > a.stride * a.pool.page_tokens.d) bad |= ZG_STATUS_POSITION;
+    auto tiles_of = [&](uint32_t r) {
+        const int n = a.lengths[r];
+        const uint32_t room = a.stride * a.pool.page_tokens.d;
+        if (n > 0 && (uint32_t)n > room) bad |= ZG_STATUS_POSITION;
+        return n < 0 ? 0u : (min((uint32_t)n, room) + F::kTile - 1) / F::kTile;
+    };
+    auto sum_upto = [&](uint32_t x) {  // of this lane and the ones before it
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t y = (uint32_t)__shfl_up((int)x, off, kWave);
+            if (lane >= off) x += y;
+        }
+        return x;
+    };
+    uint32_t all;
+    if (a.rows <= 64) {
+        const uint32_t mine = (uint32_t)lane < a.rows ? tiles_of(lane) : 0, upto = sum_upto(mine);
+        if ((uint32_t)lane < a.rows) ahead[lane] = upto - mine;
+        all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        if (lane == 0) ahead[a.rows] = all;
+        same_wave();
+    } else {
+        uint32_t* sums = ahead + a.rows + 1;
+        const uint32_t per = (a.rows + 64 * WAVES - 1) / (64 * WAVES), r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
+        uint32_t mine = 0;
+        for (uint32_t r = r0; r < r1; ++r) mine += tiles_of(r);
+        const uint32_t upto = sum_upto(mine);
+        if (lane == 63) sums[wave] = upto;
+        __syncthreads();
+        uint32_t at = upto - mine;
+        for (int w = 0; w < wave; ++w) at += sums[w];
+        for (uint32_t r = r0; r < r1; ++r) {
+            ahead[r] = at;
+            at += tiles_of(r);
+        }
+        all = 0;
+        for (int w = 0; w < WAVES; ++w) all += sums[w];
+        if (tid == 0) ahead[a.rows] = all;
+        __syncthreads();
     }
     if (bad && a.status && id == 0) atomicOr(a.status, bad);
-    uint32_t upto = mine;  // inclusive sum over the wave, then over the waves
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t x = (uint32_t)__shfl_up((int)upto, off, kWave);
-        if (lane >= off) upto += x;
-    }
-    if (lane == 63) sums[wave] = upto;
-    __syncthreads();
-    uint32_t at = upto - mine;
-    for (int w = 0; w < wave; ++w) at += sums[w];
-    for (uint32_t r = tid * per; r < min((tid + 1) * per, a.rows); ++r) {
-        ahead[r] = at;
-        at += own_tiles<F::kTile>(a, r);
-    }
-    const uint32_t all = sums[0] + sums[1] + sums[2] + sums[3];
-    if (tid == 0) ahead[a.rows] = all;
-    __syncthreads();
     const uint32_t kvs = a.pool.kv_heads, total = all * kvs;
     const uint32_t run = (total + c.waves - 1) / c.waves;
+    if (id == groups - 1)  // for the join; the last workgroup has the least to do
+        for (uint32_t i = tid; i < a.rows * kvs; i += 64 * WAVES) {
+            const uint32_t r = i / kvs, n = ahead[r + 1] - ahead[r], t = ahead[r] * kvs + (i - r * kvs) * n;
+            c.runs[i] = n ? make_uint2(t / run, (t + n - 1) / run - t / run + 1) : make_uint2(0, 0);
+        }
     // neighbouring runs lie on different CUs
     const uint32_t w = wave * groups + id;
     uint32_t t = w * run;
     const uint32_t end = min(t + run, total);
-    if (t >= end) return;
+    if (wave >= c.per_group || t >= end) return;
     // the row that holds tile t: the last one with ahead[row] * kvs <= t
     uint32_t r = 0;
     for (uint32_t lo = 0, hi = a.rows; hi - lo > 1;) {
@@ -440,7 +535,7 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
         if (ahead[mid] * kvs <= t) lo = r = mid;
         else hi = mid;
     }
-    v4u* queries = (v4u*)(lds + (((a.rows + 5) * 4 + 15) & ~15u)) + wave * F::kParts * F::kSteps * 4 * a.group;
+    v4u* queries = (v4u*)(lds + table_bytes(a.rows, WAVES)) + wave * F::kParts * F::kSteps * 4 * a.group;
     bad = 0;
     while (t < end) {
         const uint32_t n = ahead[r + 1] - ahead[r];
@@ -456,9 +551,7 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
             __device__ size_t operator()(int m) const { return first + (size_t)m * D; }
         } who{a.q, r * a.q_stride + (size_t)kvh * a.group * D};
         stage_queries<IO, KV, D>(queries, a.group, lane, 64, who);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        same_wave();
         Sums<D, 1> s;
         s.clear();
         add_tiles<IO, KV, D, 1>(a, queries, a.group, a.table + (size_t)r * a.stride, own_tokens(a, r), (int)tile,
@@ -474,77 +567,217 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
     if (bad && a.status) atomicOr(a.status, bad);
 }
 
+// Few queries over the prefix (16 MT a pass): it is bound by memory, so the
+// four waves take tiles of their own, straight into registers.
 template <bool IO, bool KV, int D, int MT>
-__global__ __launch_bounds__(256, MT * D > 128 ? 1 : 2) void paged_attn_kernel(PagedAttnArgs a, Cut c) {
+__global__ __launch_bounds__(256, MT * D > 256 ? 1 : 2) void paged_attn_kernel(PagedAttnArgs a, Cut c) {
     extern __shared__ __align__(16) char lds[];
     const int over_prefix = c.chunks * c.blocks * a.pool.kv_heads;
     if ((int)blockIdx.x < over_prefix) prefix_block<IO, KV, D, MT>(a, c, blockIdx.x, lds);
-    else own_block<IO, KV, D>(a, c, blockIdx.x - over_prefix, lds);
+    else own_block<IO, KV, D, 4>(a, c, blockIdx.x - over_prefix, lds);
 }
 
-// Workgroup (query head, row, 64 elements): lane group tid / 16 joins the
-// pieces tid / 16, + 16, ... in their order, the prefix's first.
-template <bool IO, int D, int TILE>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c, int mt) {
-    extern __shared__ float weight[];  // per piece
-    __shared__ uint32_t sums[2][4];
-    __shared__ float tops[4], ls[4];
+constexpr int kManyWaves = 8, kManyQueries = 16 * kManyWaves;
+
+// Many queries over the prefix: each of eight waves holds 16 queries and their
+// sums in registers, and all go through the same tiles, which are copied
+// straight to LDS one tile ahead; a tile is read from memory once for 128
+// queries.  In LDS the 16-byte pieces of row t are exchanged by an xor of t,
+// so that 16 lanes reading one piece of 16 rows meet 16 different banks.
+template <bool IO, bool KV, int D>
+__device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
+    using F = Form<IO, KV, D>;
+    constexpr int W = F::kWide, H = F::kHalves, N = F::kMine;
+    constexpr int ES = KV ? 2 : 4, VR = W * ES / 4;
+    constexpr int kRow = D * ES, kPieces = kRow / 16;   // bytes and 16-byte pieces of a row
+    constexpr int kHalf = F::kTile * kRow;              // bytes of a tile's keys; its values follow
+    constexpr int kCopies = 2 * kHalf / 1024 / kManyWaves;  // 1 KB each, of a wave
+    constexpr uint32_t kAll = H == 2 ? 0xffffffffu : 0xffffu;
+    const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const float to_log2 = a.scale * 1.44269504088896341f;
+    const PieceOf at_piece = piece_of(c, a.pool.kv_heads, id);
+    const int kvh = at_piece.kvh, queries = (int)a.rows * a.group;
+    const int first = at_piece.chunk * c.chunk_tiles, end = min(first + c.chunk_tiles, c.prefix_tiles);
+    auto swizzle = [](int row) { return kPieces >= 16 ? row & 15 : row >> 1 & 7; };
+    // where this lane reads: its first piece of a key row and of a value row;
+    // step i of a key is the piece xor 4 i, value row j the piece xor j
+    int key_at = col * kRow + 16 * (quarter ^ swizzle(col));
+    int value_at = kHalf + 4 * quarter * kRow +
+                   (VR == 4 ? 16 * (col ^ swizzle(4 * quarter)) : 16 * ((col >> 1) ^ swizzle(4 * quarter)) + 8 * (col & 1));
+
+    // Addresses are formed anew for each tile (the empty asm keeps them from
+    // being held): registers are short, and a spilled one, reloaded, would
+    // wait for the copies under way.
+    auto copy = [&](const Place& at, int buffer) {
+        int self = lane;
+        asm volatile("" : "+v"(self));
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int x = wave * kCopies + i, within = (x * 1024 & (kHalf - 1)) / 16 + self;
+            const int row = within / kPieces, piece = within % kPieces ^ swizzle(row);
+            const char* from = (const char*)(x * 1024 < kHalf ? a.pool.keys : a.pool.values) +
+                               ((uint64_t)(uint32_t)__shfl((int)at.unit, row) * 64 + (uint32_t)kvh * D) * ES + 16 * piece;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(lds + buffer * 2 * kHalf + x * 1024),
+                                             16, 0, 0);
+        }
+    };
+
+    // the wave's queries, in operand order
+    const int mine = at_piece.block * kManyQueries + 16 * wave + col, f = min(mine, queries - 1), r = f / a.group;
+    const size_t from = r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
+    const bool live = at_piece.block * kManyQueries + 16 * wave < queries;
+    Place at = resolve<F::kTile>(a.pool, peek<F::kTile>(a.pool, a.prefix, a.prefix_tokens, first, lane), a.prefix_tokens,
+                                 first, lane);
+    copy(at, 0);
+    uint32_t page = peek<F::kTile>(a.pool, a.prefix, a.prefix_tokens, first + 1, lane);
+    v4u q[F::kParts][F::kSteps];
+#pragma unroll
+    for (int i = 0; i < F::kSteps; ++i) {
+        if constexpr (!KV) {
+            q[0][i] = __builtin_bit_cast(v4u, load4<IO>(a.q, from + 16 * i + 4 * quarter));
+        } else if constexpr (IO) {
+            q[0][i] = *(const v4u*)((const uint16_t*)a.q + from + 32 * i + 8 * quarter);
+        } else {
+            v4f x[2] = {load4<false>(a.q, from + 32 * i + 8 * quarter), load4<false>(a.q, from + 32 * i + 8 * quarter + 4)};
+#pragma unroll
+            for (int p = 0; p < F::kParts; ++p) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[p][i][j] = pack_high(x[j >> 1][(2 * j) & 3], x[j >> 1][(2 * j + 1) & 3]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j >> 2][j & 3] -= high_part(x[j >> 2][j & 3]);
+            }
+        }
+    }
+    Sums<D, 1> s;
+    s.clear();
+    int bad = 0;
+    for (int tile = first; tile < end; ++tile) {
+        if (at.stray) bad |= ZG_STATUS_PAGE;
+        const uint32_t there = (uint32_t)__ballot(at.ok) & kAll;
+        const int buffer = (tile - first) & 1;
+        // this wave's copies have landed; after the barrier everyone's, and
+        // the other buffer has been read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (tile + 1 < end) {
+            at = resolve<F::kTile>(a.pool, page, a.prefix_tokens, tile + 1, lane);
+            copy(at, buffer ^ 1);
+            page = peek<F::kTile>(a.pool, a.prefix, a.prefix_tokens, tile + 2, lane);
+        }
+        if (!live) continue;
+        const char* const data = lds + buffer * 2 * kHalf;
+        asm volatile("" : "+v"(key_at), "+v"(value_at));
+        v4f sc[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) sc[h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < F::kSteps; ++i) {
+            v4u k[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) k[h] = *(const v4u*)(data + (key_at ^ 64 * (i & 3)) + 16 * h * kRow + 256 * (i / 4));
+#pragma unroll
+            for (int p = 0; p < F::kParts; ++p)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    if constexpr (KV) {
+                        sc[h] = mfma_bf16(k[h], q[p][i], sc[h]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h][e]),
+                                                                         __uint_as_float(q[0][i][e]), sc[h], 0, 0, 0);
+                    }
+                }
+        }
+        float w[1][N];
+        weigh<IO, KV, D, 1>((const v4f(&)[1][H])sc, there, to_log2, quarter, s, w);
+#pragma unroll
+        for (int g = 0; g < F::kLoads; ++g) {
+            uint32_t v[N][VR];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int exchange = 16 * (kPieces >= 16 ? j & 3 : (j & 3) >> 1);
+                const char* from = data + (value_at ^ exchange) + (16 * (j >> 2) + (j & 3)) * kRow + 256 * g;
+                if constexpr (VR == 4) {
+                    const v4u x = *(const v4u*)from;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) v[j][y] = x[y];
+                } else {
+                    const uint2 x = *(const uint2*)from;
+                    v[j][0] = x.x;
+                    v[j][1] = x.y;
+                }
+            }
+            drop_values<KV>(v, there, quarter);
+            add_values<IO, KV, D, 1>(v, w, g, s);
+        }
+    }
+    if (bad && a.status) atomicOr(a.status, bad);
+    s.l[0] += __shfl_xor(s.l[0], 16, kWave);
+    s.l[0] += __shfl_xor(s.l[0], 32, kWave);
+    if (mine < queries)
+        store_sums<W, D>(c.prefix_stats, c.prefix_o,
+                         ((size_t)(kvh * c.chunks + at_piece.chunk) * c.blocks) * kManyQueries + mine, s.o[0], s.ref[0],
+                         s.l[0], quarter);
+}
+
+template <bool IO, bool KV, int D>
+__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_attn_many_kernel(PagedAttnArgs a, Cut c) {
+    extern __shared__ __align__(16) char lds[];
+    const int over_prefix = c.chunks * c.blocks * a.pool.kv_heads;
+    if ((int)blockIdx.x < over_prefix) many_block<IO, KV, D>(a, c, blockIdx.x, lds);
+    else own_block<IO, KV, D, kManyWaves>(a, c, blockIdx.x - over_prefix, lds);
+}
+
+// Workgroup (query head, row, 64 elements): 16 lanes hold the elements, the
+// 16 lane groups of the four waves join pieces g, g + 16, ... in order, the
+// prefix's first, then the groups are added in order.  Every wave reads all
+// pieces' m and l itself, so nothing waits for a barrier before the sums.
+template <bool IO, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c) {
     __shared__ v4f parts[16][16];
     const uint32_t h = blockIdx.x, r = blockIdx.y;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (a.lengths[r] < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t kvs = a.pool.kv_heads, kvh = h / a.group, in_group = h - kvh * a.group;
-    uint32_t before = 0, all = 0;
-    for (uint32_t i = tid; i < a.rows; i += 256) {
-        const uint32_t n = own_tiles<TILE>(a, i);
-        all += n;
-        if (i < r) before += n;
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        before += (uint32_t)__shfl_xor((int)before, off, kWave);
-        all += (uint32_t)__shfl_xor((int)all, off, kWave);
-    }
-    if (lane == 0) {
-        sums[0][wave] = before;
-        sums[1][wave] = all;
-    }
-    __syncthreads();
-    before = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
-    all = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-    const uint32_t run = (all * kvs + c.waves - 1) / c.waves, n = own_tiles<TILE>(a, r);
-    const uint32_t tile = before * kvs + kvh * n;
-    const uint32_t first = n ? tile / run : 0, own = n ? (tile + n - 1) / run - first + 1 : 0;
-    const uint32_t pieces = c.chunks + own;
-    const uint32_t f = r * a.group + in_group;
-    auto prefix_at = [&](uint32_t i) { return ((size_t)(kvh * c.chunks + i) * c.blocks) * 16 * mt + f; };
-    auto own_at = [&](uint32_t i) { return ((size_t)first + i + r * kvs + kvh) * a.group + in_group; };
-    float top = -INFINITY;
-    for (uint32_t i = tid; i < pieces; i += 256)
-        top = fmaxf(top, i < (uint32_t)c.chunks ? c.prefix_stats[prefix_at(i)].x : c.own_stats[own_at(i - c.chunks)].x);
-    top = wave_max(top);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const float sub = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
-    for (uint32_t i = tid; i < pieces; i += 256) {
-        const float2 x = i < (uint32_t)c.chunks ? c.prefix_stats[prefix_at(i)] : c.own_stats[own_at(i - c.chunks)];
-        const float e = __builtin_amdgcn_exp2f(x.x == top ? 0.0f : x.x - sub);
-        weight[i] = e;
-        l += e * x.y;
-    }
-    l = wave_sum_xor(l, kWave);
-    if (lane == 0) ls[wave] = l;
-    __syncthreads();
-    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    const int e = blockIdx.z * 64 + 4 * (tid & 15);
+    const uint2 run = c.runs[r * kvs + kvh];  // first wave, pieces
+    if (a.lengths[r] < 0) return;
+    const uint32_t chunks = c.chunks, pieces = chunks + run.y;
+    const size_t prefix_at = (size_t)kvh * c.chunks * c.blocks * c.block + r * a.group + in_group;
+    const size_t prefix_step = (size_t)c.blocks * c.block;
+    const size_t own_at = ((size_t)run.x + r * kvs + kvh) * a.group + in_group;
+    const int e = blockIdx.z * 64 + 4 * (tid & 15), g = tid >> 4;
+    auto stats = [&](uint32_t i) {
+        return i < chunks ? c.prefix_stats[prefix_at + i * prefix_step] : c.own_stats[own_at + (size_t)(i - chunks) * a.group];
+    };
+    auto elements = [&](uint32_t i) {
+        return *(const v4f*)((i < chunks ? c.prefix_o + (prefix_at + i * prefix_step) * D
+                                         : c.own_o + (own_at + (size_t)(i - chunks) * a.group) * D) + e);
+    };
+    float top = -INFINITY, l = 0.0f;
     v4f o = {};
-    for (uint32_t i = tid >> 4; i < pieces; i += 16) {
-        const float* from = i < (uint32_t)c.chunks ? c.prefix_o + prefix_at(i) * D : c.own_o + own_at(i - c.chunks) * D;
-        o += weight[i] * *(const v4f*)(from + e);
+    // 64 pieces at a time, the sums brought to the highest m so far
+    for (uint32_t from = 0; from < pieces; from += 64) {
+        const uint32_t n = min(64u, pieces - from);
+        // this lane's piece of the 64, and the lane group's four
+        const float2 x = (uint32_t)lane < n ? stats(from + lane) : make_float2(-INFINITY, 0.0f);
+        v4f p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (g + 16 * u < n) p[u] = elements(from + g + 16 * u);
+        const float to = fmaxf(top, wave_max(x.x)), sub = to == -INFINITY ? 0.0f : to;
+        const float keep = __builtin_amdgcn_exp2f(top == to ? 0.0f : top - sub);
+        const float w = __builtin_amdgcn_exp2f(x.x == to ? 0.0f : x.x - sub);
+        l = l * keep + wave_sum_xor((uint32_t)lane < n ? w * x.y : 0.0f, kWave);
+        o *= keep;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float wu = __shfl(w, g + 16 * u, kWave);
+            if (g + 16 * u < n) o += wu * p[u];
+        }
+        top = to;
     }
-    parts[tid >> 4][tid & 15] = o;
+    parts[g][tid & 15] = o;
     __syncthreads();
     if (tid >= 16) return;
     o = parts[0][tid];
@@ -557,28 +790,33 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c,
 
 // ------------------------------------------------------------------- host
 
-// Tiles of 16 queries that share a pass over the prefix: their sums take
-// MT * D / 4 registers a lane of the 512.
-static int tiles_of_queries(uint32_t rows, int group, int head_dim) {
+// Queries of one kv head that go over the prefix in one pass: 16 or 32 in a
+// wave, or 128 in a workgroup.
+static int block_of(uint32_t rows, int group) {
     const uint64_t n = (uint64_t)rows * group;
-    return n <= 16 ? 1 : n <= 32 || head_dim == 256 ? 2 : 4;
+    return n <= 16 ? 16 : n <= 32 ? 32 : kManyQueries;
 }
 
 static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int tile, uint32_t prefix_tokens,
-                  uint64_t row_tokens, void* workspace, size_t* bytes) {
+                  uint64_t row_tokens, size_t query_bytes, void* workspace, size_t* bytes) {
     Cut c{};
-    const int group = q_heads / kv_heads, mt = tiles_of_queries(rows, group, head_dim);
-    c.blocks = (int)(((uint64_t)rows * group + 16 * mt - 1) / (16 * mt));
+    const int group = q_heads / kv_heads;
+    c.block = block_of(rows, group);
+    c.blocks = (int)(((uint64_t)rows * group + c.block - 1) / c.block);
     c.prefix_tiles = (int)((prefix_tokens + tile - 1) / tile);
     if (c.prefix_tiles) {
-        const int most = (c.prefix_tiles + 3) / 4;  // four tiles: one a wave
-        const int want = std::max(1, std::min(most, kPrefixGroups / std::max(1, kv_heads * c.blocks)));
+        const int least = c.block == kManyQueries ? kManyTiles : 4;  // tiles of a piece
+        const int want = std::max(1, std::min((c.prefix_tiles + least - 1) / least,
+                                              kPrefixGroups / std::max(1, kv_heads * c.blocks)));
         c.chunk_tiles = (c.prefix_tiles + want - 1) / want;
         c.chunks = (c.prefix_tiles + c.chunk_tiles - 1) / c.chunk_tiles;
     }
+    // eight waves' queries may not fit the LDS (16 to a kv head, in three parts)
+    const bool many = c.chunks && c.block == kManyQueries;
+    c.per_group = many && kManyWaves * group * query_bytes <= kOwnLds ? kManyWaves : 4;
     const uint64_t own_tiles = (uint64_t)rows * kv_heads * ((row_tokens + tile - 1) / tile);
-    c.waves = 4 * (int)std::min<uint64_t>(kOwnGroups, own_tiles);
-    const size_t prefix_rows = (size_t)kv_heads * c.chunks * c.blocks * 16 * mt;
+    c.waves = c.per_group * (int)std::min<uint64_t>(kOwnWaves / c.per_group, own_tiles);
+    const size_t prefix_rows = (size_t)kv_heads * c.chunks * c.blocks * c.block;
     const size_t own_rows = ((size_t)c.waves + (size_t)rows * kv_heads) * group;
     char* at = (char*)workspace;
     auto take = [&](size_t n) {
@@ -586,6 +824,7 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
         at += (n + 255) / 256 * 256;
         return p;
     };
+    c.runs = (uint2*)take((size_t)rows * kv_heads * sizeof(uint2));
     c.prefix_stats = (float2*)take(prefix_rows * sizeof(float2));
     c.own_stats = (float2*)take(own_rows * sizeof(float2));
     c.prefix_o = (float*)take(prefix_rows * head_dim * sizeof(float));
@@ -597,46 +836,51 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
 size_t paged_attn_workspace(uint32_t rows, int q_heads, int kv_heads, int head_dim, int bf16, uint32_t prefix_tokens,
                             uint64_t row_tokens) {
     size_t bytes = 0;
-    cut_of(rows, q_heads, kv_heads, head_dim, bf16 ? 32 : 16, prefix_tokens, row_tokens, nullptr, &bytes);
+    // no call leaves more pieces than one whose queries take the least room
+    cut_of(rows, q_heads, kv_heads, head_dim, bf16 ? 32 : 16, prefix_tokens, row_tokens, 0, nullptr, &bytes);
     return bytes;
 }
 
-template <bool IO, bool KV, int D, int MT>
-static hipError_t launch(const PagedAttnArgs& a, const Cut& c, hipStream_t st) {
+// A staged query: 16 bytes for each part, step and quarter.
+template <bool IO, bool KV, int D>
+constexpr size_t query_bytes() {
+    return (size_t)Form<IO, KV, D>::kParts * Form<IO, KV, D>::kSteps * 4 * 16;
+}
+
+template <bool IO, bool KV, int D>
+static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
+    const Cut c = cut_of(a.rows, a.q_heads, a.pool.kv_heads, D, Form<IO, KV, D>::kTile, a.prefix_tokens,
+                         (uint64_t)a.stride * a.pool.page_tokens.d, query_bytes<IO, KV, D>(), a.workspace, nullptr);
     using F = Form<IO, KV, D>;
-    const size_t queries = (size_t)F::kParts * F::kSteps * 4 * 16;  // bytes of a query, 16 a step and part and quarter
-    const size_t prefix = c.chunks ? std::max(queries * 16 * MT, (size_t)4 * 16 * MT * 8 + (size_t)2 * MT * D * 64) : 0;
-    const size_t own = ((a.rows + 5) * 4 + 15) / 16 * 16 + 4 * a.group * queries;
+    const bool many = c.chunks && c.block == kManyQueries;
+    const int waves = many ? kManyWaves : 4;
+    constexpr size_t query = query_bytes<IO, KV, D>();
+    const size_t own = table_bytes(a.rows, waves) + c.per_group * a.group * query;
+    size_t prefix = 0;
+    if (many) prefix = (size_t)4 * F::kTile * D * (KV ? 2 : 4);  // two tiles' keys and values
+    else if (c.chunks) prefix = std::max(query * c.block, (size_t)4 * c.block * 8 + (size_t)2 * c.block * D * 4);
     const size_t lds = std::max(prefix, own);
-    auto kernel = paged_attn_kernel<IO, KV, D, MT>;
+    void (*kernel)(PagedAttnArgs, Cut) = many                            ? paged_attn_many_kernel<IO, KV, D>
+                                         : c.chunks && c.block == 32 ? paged_attn_kernel<IO, KV, D, 2>
+                                                                         : paged_attn_kernel<IO, KV, D, 1>;
     if (lds > 65536) {
         hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    kernel<<<c.chunks * c.blocks * a.pool.kv_heads + c.waves / 4, 256, lds, st>>>(a, c);
+    kernel<<<c.chunks * c.blocks * a.pool.kv_heads + c.waves / c.per_group, 64 * waves, lds, st>>>(a, c);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    paged_join_kernel<IO, D, F::kTile><<<dim3(a.q_heads, a.rows, D / 64), 256, (c.chunks + c.waves) * sizeof(float), st>>>(a, c, MT);
+    paged_join_kernel<IO, D><<<dim3(a.q_heads, a.rows, D / 64), 256, 0, st>>>(a, c);
     return hipGetLastError();
 }
 
 hipError_t paged_attn(const PagedAttnArgs& a, hipStream_t st) {
-    const Cut c = cut_of(a.rows, a.q_heads, a.pool.kv_heads, a.pool.head_dim, a.pool.bf16 ? 32 : 16, a.prefix_tokens,
-                         (uint64_t)a.stride * a.pool.page_tokens.d, a.workspace, nullptr);
-    const int mt = c.chunks ? tiles_of_queries(a.rows, a.group, a.pool.head_dim) : 1;
-    auto by_tiles = [&](auto io, auto kv, auto dim) {
-        constexpr bool IO = decltype(io)::value, KV = decltype(kv)::value;
-        constexpr int D = decltype(dim)::value;
-        if (mt == 1) return launch<IO, KV, D, 1>(a, c, st);
-        if constexpr (D < 256)
-            if (mt == 4) return launch<IO, KV, D, 4>(a, c, st);
-        return launch<IO, KV, D, 2>(a, c, st);
-    };
     auto by_dim = [&](auto io, auto kv) {
+        constexpr bool IO = decltype(io)::value, KV = decltype(kv)::value;
         switch (a.pool.head_dim) {
-        case 64: return by_tiles(io, kv, std::integral_constant<int, 64>{});
-        case 128: return by_tiles(io, kv, std::integral_constant<int, 128>{});
-        default: return by_tiles(io, kv, std::integral_constant<int, 256>{});
+        case 64: return launch<IO, KV, 64>(a, st);
+        case 128: return launch<IO, KV, 128>(a, st);
+        default: return launch<IO, KV, 256>(a, st);
         }
     };
     if (a.io_bf16) return a.pool.bf16 ? by_dim(std::true_type{}, std::true_type{}) : by_dim(std::true_type{}, std::false_type{});
