@@ -32,6 +32,7 @@ constexpr int kOwnWaves = 2048;     // waves over the rows' own tiles: two per S
 constexpr int kManyTiles = 2;       // fewest tiles of a piece of the prefix for 128 queries
 constexpr int kPrefixGroups = 256;  // about so many over the prefix
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
+constexpr int kJoin = 8;             // pieces that a thread of the join has under way
 constexpr float kRaise = 8.0f;      // log2: how far a score may pass the reference before sums are rescaled
 
 template <bool IO, bool KV, int D>
@@ -195,16 +196,24 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const flo
                 for (int j = 0; j < 8; ++j) x[j] -= high_part(x[j]);
             }
         }
+        // two accumulators at a time: a product waits for the one before it on
+        // the same accumulator (four would not leave the registers for it)
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            v4u rows;
+        for (int from = 0; from < W; from += 2) {
+            v4u rows[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                rows[j] = __builtin_amdgcn_perm(v[2 * j + 1][i >> 1], v[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    rows[i][j] = __builtin_amdgcn_perm(v[2 * j + 1][(from + i) >> 1], v[2 * j][(from + i) >> 1],
+                                                       i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
             for (int p = 0; p < F::kWeightParts; ++p)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) s.o[m][g * W + i] = mfma_bf16(rows, part[m][p], s.o[m][g * W + i]);
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                        s.o[m][g * W + from + i] = mfma_bf16(rows[i], part[m][p], s.o[m][g * W + from + i]);
         }
     } else {
 #pragma unroll
@@ -318,33 +327,118 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
     }
 }
 
-// One triple per query: m and l side by side, then the D elements.
-template <int W, int D>
-__device__ __forceinline__ void store_sums(float2* stats, float* o, size_t at, const v4f (&from)[D / 16], float ref,
-                                           float l, int quarter) {
-    if (quarter == 0) stats[at] = make_float2(ref, l);
+// One triple per query: m and l side by side; the elements of `across`
+// queries together in the order of the sums, 16 bytes per (accumulator,
+// quarter, query), so that a wave stores whole lines.
+template <int D>
+__device__ __forceinline__ void store_sums(float2* stats, float* o, int across, int query, const v4f (&from)[D / 16],
+                                           float ref, float l, int quarter) {
+    if (quarter == 0) stats[query] = make_float2(ref, l);
+    int at = (quarter * across + query) * 4;  // formed here, not held through the tiles
+    asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int g = 0; g < D / (16 * W); ++g)
+    for (int f = 0; f < D / 16; ++f) *(v4f*)(o + f * 16 * across + at) = from[f];
+}
+
+// The sums of waves 0 .. n - 1 brought together in wave 0, in a fixed order;
+// every wave of the workgroup calls this.
+template <int D, int MT>
+__device__ __forceinline__ void gather_waves(Sums<D, MT>& s, int n, int wave, int lane, char* lds) {
+    const int quarter = lane >> 4, col = lane & 15;
+    float2* stats = (float2*)lds;  // [n][16 MT]
+    v4f* part = (v4f*)(lds + n * 16 * MT * sizeof(float2));
+    const bool mine = wave < n;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+    for (int m = 0; m < MT; ++m) {
+        s.l[m] += __shfl_xor(s.l[m], 16, kWave);
+        s.l[m] += __shfl_xor(s.l[m], 32, kWave);
+        if (mine && quarter == 0) stats[wave * 16 * MT + 16 * m + col] = make_float2(s.ref[m], s.l[m]);
+    }
+    __syncthreads();
 #pragma unroll
-            for (int x = 0; x < W; x += 4)
-                *(v4f*)(o + at * D + 16 * W * g + W * (4 * quarter + r) + x) =
-                    v4f{from[g * W + x][r], from[g * W + x + 1][r], from[g * W + x + 2][r], from[g * W + x + 3][r]};
+    for (int m = 0; m < MT; ++m) {
+        float top = -INFINITY;
+        for (int w = 0; w < n; ++w) top = fmaxf(top, stats[w * 16 * MT + 16 * m + col].x);
+        const float sub = top == -INFINITY ? 0.0f : top;
+        s.l[m] = 0.0f;
+        for (int w = 0; w < n; ++w) {
+            const float2 x = stats[w * 16 * MT + 16 * m + col];
+            s.l[m] += x.y * __builtin_amdgcn_exp2f(x.x == top ? 0.0f : x.x - sub);
+        }
+        const float keep = __builtin_amdgcn_exp2f(s.ref[m] == top ? 0.0f : s.ref[m] - sub);
+        s.ref[m] = top;
+#pragma unroll
+        for (int f = 0; f < D / 16; ++f) s.o[m][f] *= keep;
+    }
+    while (n > 1) {
+        const int half = (n + 1) / 2;
+        if (wave >= half && wave < n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int f = 0; f < D / 16; ++f) part[(((wave - half) * MT + m) * (D / 16) + f) * 64 + lane] = s.o[m][f];
+        __syncthreads();
+        if (wave < n - half)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int f = 0; f < D / 16; ++f) s.o[m][f] += part[((wave * MT + m) * (D / 16) + f) * 64 + lane];
+        __syncthreads();
+        n = half;
+    }
+}
+constexpr size_t gather_bytes(int waves, int mt, int head_dim) {
+    return (size_t)waves * 16 * mt * sizeof(float2) + (size_t)(waves / 2) * mt * head_dim * 64;
 }
 
 // How a call is cut.  The prefix: `chunks` pieces of chunk_tiles tiles, each
 // for `blocks` blocks of `block` queries and every kv head.  The rows' own
-// tiles, in the order (row, kv head, tile): wave w of the `waves` takes c
-// successive ones, c = ceil(all / waves), whatever rows they belong to, so
-// that long and short rows fill the card alike; where a wave's run crosses
-// from one (row, kv head) to the next it leaves one triple for each.
+// tiles, in the order (row, kv head, tile), go in runs of `run` successive
+// ones to the waves, `active` waves of each of the `groups` workgroups,
+// whatever rows they belong to, so that long and short rows fill the card
+// alike.  Where a workgroup's runs lie within one (row, kv head) its waves'
+// sums are gathered to one piece; else each wave leaves a piece for each (row,
+// kv head) that it meets.
 struct Cut {
-    int prefix_tiles, chunk_tiles, chunks, block, blocks, waves, per_group;  // per_group of the waves in a workgroup
-    uint2* runs;  // per (row, kv head): its first wave and how many hold a piece of it
+    int prefix_tiles, chunk_tiles, chunks, block, blocks, groups, per_group;  // per_group: most waves of a workgroup
+    struct Run* runs;
     float2 *prefix_stats, *own_stats;
     float *prefix_o, *own_o;
 };
+// The pieces of one (row, kv head), by the waves that leave them: heads of
+// successive waves, then mids of every `active`-th (gathered workgroups), then
+// tails of successive waves.
+struct Run {
+    uint32_t head, heads, mid, mids, tail, tails, active;
+};
+struct Shares {
+    uint32_t active, run, total;
+};
+__host__ __device__ inline Shares shares_of(uint32_t total, uint32_t groups, uint32_t per_group) {
+    Shares s;
+    const uint32_t each = (total + groups - 1) / groups;
+    s.active = each < 1 ? 1 : each < per_group ? each : per_group;
+    s.run = (total + groups * s.active - 1) / (groups * s.active);
+    s.total = total;
+    return s;
+}
+__device__ __forceinline__ Run run_of(const Shares& s, uint32_t from, uint32_t to) {
+    Run r{0, 0, 0, 0, 0, 0, s.active};
+    if (from == to) return r;
+    const uint32_t whole = s.active * s.run, g0 = (from + whole - 1) / whole;
+    const uint32_t g1 = to == s.total ? (to + whole - 1) / whole : to / whole;
+    r.head = from / s.run;
+    if (g0 >= g1) {
+        r.heads = (to - 1) / s.run - r.head + 1;
+        return r;
+    }
+    if (from < g0 * whole) r.heads = g0 * s.active - r.head;
+    r.mid = g0 * s.active;
+    r.mids = g1 - g0;
+    r.tail = g1 * s.active;
+    if (to > g1 * whole) r.tails = (to - 1) / s.run - r.tail + 1;
+    return r;
+}
 
 __device__ __forceinline__ uint32_t own_tokens(const PagedAttnArgs& a, uint32_t r) {
     const int n = a.lengths[r];
@@ -374,8 +468,8 @@ __device__ __forceinline__ PieceOf piece_of(const Cut& c, int kv_heads, int id) 
 
 template <bool IO, bool KV, int D, int MT>
 __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
-    using F = Form<IO, KV, D>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PieceOf at_piece = piece_of(c, a.pool.kv_heads, id);
     const int block = at_piece.block, kvh = at_piece.kvh, chunk = at_piece.chunk;
     const int queries = (int)a.rows * a.group;
@@ -398,59 +492,14 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
                              min(first + c.chunk_tiles, c.prefix_tiles), 4, kvh, s, bad);
     if (bad && a.status) atomicOr(a.status, bad);
     __syncthreads();
-    // the four waves' sums: the common reference, then o in pairs
-    float2* stats = (float2*)lds;  // [4][16 MT]
-    v4f* part = (v4f*)(lds + 4 * 16 * MT * sizeof(float2));
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        s.l[m] += __shfl_xor(s.l[m], 16, kWave);
-        s.l[m] += __shfl_xor(s.l[m], 32, kWave);
-        if (quarter == 0) stats[wave * 16 * MT + 16 * m + col] = make_float2(s.ref[m], s.l[m]);
-    }
-    __syncthreads();
-    float ref[MT], l[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        float2 x[4];
-        ref[m] = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            x[w] = stats[w * 16 * MT + 16 * m + col];
-            ref[m] = fmaxf(ref[m], x[w].x);
-        }
-        const float sub = ref[m] == -INFINITY ? 0.0f : ref[m];
-        l[m] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) l[m] += x[w].y * __builtin_amdgcn_exp2f(x[w].x == ref[m] ? 0.0f : x[w].x - sub);
-        const float mine = __builtin_amdgcn_exp2f(s.ref[m] == ref[m] ? 0.0f : s.ref[m] - sub);
-#pragma unroll
-        for (int f = 0; f < F::kFrags; ++f) s.o[m][f] *= mine;
-    }
-    auto put = [&](int to) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int f = 0; f < F::kFrags; ++f) part[((to * MT + m) * F::kFrags + f) * 64 + lane] = s.o[m][f];
-    };
-    auto add = [&](int from) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int f = 0; f < F::kFrags; ++f) s.o[m][f] += part[((from * MT + m) * F::kFrags + f) * 64 + lane];
-    };
-    if (wave >= 2) put(wave - 2);
-    __syncthreads();
-    if (wave < 2) add(wave);
-    __syncthreads();
-    if (wave == 1) put(0);
-    __syncthreads();
+    gather_waves<D, MT>(s, 4, wave, lane, lds);
     if (wave) return;
-    add(0);
-    const size_t at = ((size_t)(kvh * c.chunks + chunk) * c.blocks + block) * 16 * MT;
+    const size_t tile = (((size_t)kvh * c.chunks + chunk) * c.blocks + block) * MT;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
         if (block * 16 * MT + 16 * m + col < queries)
-            store_sums<F::kWide, D>(c.prefix_stats, c.prefix_o, at + 16 * m + col, s.o[m], ref[m], l[m], quarter);
+            store_sums<D>(c.prefix_stats + (tile + m) * 16, c.prefix_o + (tile + m) * 16 * D, 16, col, s.o[m], s.ref[m],
+                          s.l[m], quarter);
 }
 
 // What a wave wrote to LDS, its other lanes read after this.
@@ -468,8 +517,8 @@ __host__ __device__ inline size_t table_bytes(uint32_t rows, int waves) {
 template <bool IO, bool KV, int D, int WAVES>
 __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
     using F = Form<IO, KV, D>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
-    const int groups = c.waves / c.per_group;
+    const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // ahead[r]: tiles of the rows before r, in LDS.  Up to 64 rows every wave
     // finds them for itself, a row a lane, without a barrier; beyond, thread t
     // sums rows [t * per, (t + 1) * per).
@@ -512,38 +561,46 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
         }
         all = 0;
         for (int w = 0; w < WAVES; ++w) all += sums[w];
+        all = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
         if (tid == 0) ahead[a.rows] = all;
         __syncthreads();
     }
     if (bad && a.status && id == 0) atomicOr(a.status, bad);
-    const uint32_t kvs = a.pool.kv_heads, total = all * kvs;
-    const uint32_t run = (total + c.waves - 1) / c.waves;
-    if (id == groups - 1)  // for the join; the last workgroup has the least to do
+    const uint32_t kvs = a.pool.kv_heads;
+    const Shares share = shares_of(all * kvs, c.groups, c.per_group);
+    if (id == c.groups - 1)  // for the join; the last workgroup has the least to do
         for (uint32_t i = tid; i < a.rows * kvs; i += 64 * WAVES) {
-            const uint32_t r = i / kvs, n = ahead[r + 1] - ahead[r], t = ahead[r] * kvs + (i - r * kvs) * n;
-            c.runs[i] = n ? make_uint2(t / run, (t + n - 1) / run - t / run + 1) : make_uint2(0, 0);
+            const uint32_t r = i / kvs, n = ahead[r + 1] - ahead[r], from = ahead[r] * kvs + (i - r * kvs) * n;
+            c.runs[i] = run_of(share, from, from + n);
         }
-    // neighbouring runs lie on different CUs
-    const uint32_t w = wave * groups + id;
-    uint32_t t = w * run;
-    const uint32_t end = min(t + run, total);
-    if (wave >= c.per_group || t >= end) return;
-    // the row that holds tile t: the last one with ahead[row] * kvs <= t
+    const uint32_t w = id * share.active + wave, from = id * share.active * share.run;
+    uint32_t t = min(w * share.run, share.total);
+    const uint32_t end = (uint32_t)wave < share.active ? min(t + share.run, share.total) : t;
+    if (from >= share.total) return;
+    auto at_row = [&](uint32_t r) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)ahead[r]); };
+    // the row that holds the workgroup's first tile: the last one with
+    // ahead[row] * kvs <= from
     uint32_t r = 0;
     for (uint32_t lo = 0, hi = a.rows; hi - lo > 1;) {
         const uint32_t mid = (lo + hi) / 2;
-        if (ahead[mid] * kvs <= t) lo = r = mid;
+        if (at_row(mid) * kvs <= from) lo = r = mid;
         else hi = mid;
     }
+    // one (row, kv head) for the whole workgroup?
+    const uint32_t in_first = from - at_row(r) * kvs, tiles = at_row(r + 1) - at_row(r);
+    const uint32_t upto = min(from + share.active * share.run, share.total);
+    const bool gathered = upto - from <= tiles - in_first % tiles;
     v4u* queries = (v4u*)(lds + table_bytes(a.rows, WAVES)) + wave * F::kParts * F::kSteps * 4 * a.group;
     bad = 0;
+    Sums<D, 1> s;
+    s.clear();
     while (t < end) {
-        const uint32_t n = ahead[r + 1] - ahead[r];
-        if (ahead[r + 1] * kvs <= t) {
+        const uint32_t before = at_row(r), n = at_row(r + 1) - before;
+        if ((before + n) * kvs <= t) {
             ++r;
             continue;
         }
-        const uint32_t in_row = t - ahead[r] * kvs, kvh = in_row / n, tile = in_row - kvh * n;
+        const uint32_t in_row = t - before * kvs, kvh = in_row / n, tile = in_row - kvh * n;
         const uint32_t upto_tile = min(n, tile + (end - t));
         struct {
             const void* base;
@@ -552,19 +609,27 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
         } who{a.q, r * a.q_stride + (size_t)kvh * a.group * D};
         stage_queries<IO, KV, D>(queries, a.group, lane, 64, who);
         same_wave();
-        Sums<D, 1> s;
-        s.clear();
         add_tiles<IO, KV, D, 1>(a, queries, a.group, a.table + (size_t)r * a.stride, own_tokens(a, r), (int)tile,
                                 (int)upto_tile, 1, (int)kvh, s, bad);
         __builtin_amdgcn_wave_barrier();
+        t += upto_tile - tile;
+        if (gathered) break;
         s.l[0] += __shfl_xor(s.l[0], 16, kWave);
         s.l[0] += __shfl_xor(s.l[0], 32, kWave);
+        const size_t piece = (size_t)w + r * kvs + kvh;
         if (col < a.group)
-            store_sums<F::kWide, D>(c.own_stats, c.own_o, ((size_t)w + r * kvs + kvh) * a.group + col, s.o[0], s.ref[0],
-                                    s.l[0], quarter);
-        t += upto_tile - tile;
+            store_sums<D>(c.own_stats + piece * a.group, c.own_o + piece * a.group * D, a.group, col, s.o[0], s.ref[0],
+                          s.l[0], quarter);
+        s.clear();
     }
     if (bad && a.status) atomicOr(a.status, bad);
+    if (!gathered) return;
+    __syncthreads();
+    gather_waves<D, 1>(s, share.active, wave, lane, lds);
+    const size_t piece = (size_t)w + r * kvs + in_first / tiles;
+    if (wave == 0 && col < a.group)
+        store_sums<D>(c.own_stats + piece * a.group, c.own_o + piece * a.group * D, a.group, col, s.o[0], s.ref[0], s.l[0],
+                      quarter);
 }
 
 // Few queries over the prefix (16 MT a pass): it is bound by memory, so the
@@ -578,10 +643,12 @@ __global__ __launch_bounds__(256, MT * D > 256 ? 1 : 2) void paged_attn_kernel(P
 }
 
 constexpr int kManyWaves = 8, kManyQueries = 16 * kManyWaves;
+constexpr int kBuffers = 4, kAhead = kBuffers - 1;  // tiles in LDS, and copied ahead of the one in use
+constexpr int kSegment = 64;                        // tiles looked up at a time
 
 // Many queries over the prefix: each of eight waves holds 16 queries and their
 // sums in registers, and all go through the same tiles, which are copied
-// straight to LDS one tile ahead; a tile is read from memory once for 128
+// straight to LDS three tiles ahead; a tile is read from memory once for 128
 // queries.  In LDS the 16-byte pieces of row t are exchanged by an xor of t,
 // so that 16 lanes reading one piece of 16 rows meet 16 different banks.
 template <bool IO, bool KV, int D>
@@ -606,32 +673,52 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
     int value_at = kHalf + 4 * quarter * kRow +
                    (VR == 4 ? 16 * (col ^ swizzle(4 * quarter)) : 16 * ((col >> 1) ^ swizzle(4 * quarter)) + 8 * (col & 1));
 
+    // the places of a segment's tokens, looked up once for the workgroup; all
+    // ones: the token is not there
+    uint32_t* const units = (uint32_t*)(lds + kBuffers * 2 * kHalf);
     // Addresses are formed anew for each tile (the empty asm keeps them from
     // being held): registers are short, and a spilled one, reloaded, would
     // wait for the copies under way.
-    auto copy = [&](const Place& at, int buffer) {
+    auto copy = [&](int local, int buffer) {
         int self = lane;
         asm volatile("" : "+v"(self));
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const int x = wave * kCopies + i, within = (x * 1024 & (kHalf - 1)) / 16 + self;
             const int row = within / kPieces, piece = within % kPieces ^ swizzle(row);
+            const uint32_t unit = units[local * F::kTile + row];
             const char* from = (const char*)(x * 1024 < kHalf ? a.pool.keys : a.pool.values) +
-                               ((uint64_t)(uint32_t)__shfl((int)at.unit, row) * 64 + (uint32_t)kvh * D) * ES + 16 * piece;
+                               ((uint64_t)(unit == ~0u ? 0u : unit) * 64 + (uint32_t)kvh * D) * ES + 16 * piece;
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                              (__attribute__((address_space(3))) void*)(lds + buffer * 2 * kHalf + x * 1024),
                                              16, 0, 0);
         }
     };
+    int bad = 0;
+    auto look_up = [&](int from, int n) {
+        for (int i = threadIdx.x; i < n * F::kTile; i += 64 * kManyWaves) {
+            const uint32_t t = (uint32_t)from * F::kTile + i;
+            uint32_t unit = ~0u;
+            if (t < a.prefix_tokens) {
+                const uint32_t pg = a.pool.page_tokens.quotient(t), page = (uint32_t)a.prefix[pg];
+                if (page < a.pool.pages)
+                    unit = page * a.pool.page_units + (t - pg * a.pool.page_tokens.d) * a.pool.slot_units;
+                else
+                    bad |= ZG_STATUS_PAGE;
+            }
+            units[i] = unit;
+        }
+    };
+    int held = min(kSegment, end - first);  // tiles of the segment in `units`
+    look_up(first, held);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) copy(min(i, held - 1), i);
 
     // the wave's queries, in operand order
     const int mine = at_piece.block * kManyQueries + 16 * wave + col, f = min(mine, queries - 1), r = f / a.group;
     const size_t from = r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
     const bool live = at_piece.block * kManyQueries + 16 * wave < queries;
-    Place at = resolve<F::kTile>(a.pool, peek<F::kTile>(a.pool, a.prefix, a.prefix_tokens, first, lane), a.prefix_tokens,
-                                 first, lane);
-    copy(at, 0);
-    uint32_t page = peek<F::kTile>(a.pool, a.prefix, a.prefix_tokens, first + 1, lane);
     v4u q[F::kParts][F::kSteps];
 #pragma unroll
     for (int i = 0; i < F::kSteps; ++i) {
@@ -652,19 +739,27 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
     }
     Sums<D, 1> s;
     s.clear();
-    int bad = 0;
-    for (int tile = first; tile < end; ++tile) {
-        if (at.stray) bad |= ZG_STATUS_PAGE;
-        const uint32_t there = (uint32_t)__ballot(at.ok) & kAll;
-        const int buffer = (tile - first) & 1;
-        // this wave's copies have landed; after the barrier everyone's, and
-        // the other buffer has been read
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (tile + 1 < end) {
-            at = resolve<F::kTile>(a.pool, page, a.prefix_tokens, tile + 1, lane);
-            copy(at, buffer ^ 1);
-            page = peek<F::kTile>(a.pool, a.prefix, a.prefix_tokens, tile + 2, lane);
+    for (int tile = first, local = 0; tile < end; ++tile, ++local) {
+        if (local == held) {
+            // the next segment: everyone is done with this one, and the copies
+            // past its end have landed
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            held = min(kSegment, end - tile);
+            look_up(tile, held);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) copy(min(i, held - 1), i);
+            local = 0;
         }
+        const uint32_t there = (uint32_t)__ballot(units[local * F::kTile + (lane & (F::kTile - 1))] != ~0u) & kAll;
+        const int buffer = local % kBuffers;
+        // this tile's copies have landed when no more are under way than the
+        // later tiles'; after the barrier everyone's have, and the buffer of
+        // the tile before has been read
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kAhead - 1) * kCopies) : "memory");
+        // past the segment's last tile that one again, so that the count holds
+        copy(min(local + kAhead, held - 1), (buffer + kAhead) % kBuffers);
         if (!live) continue;
         const char* const data = lds + buffer * 2 * kHalf;
         asm volatile("" : "+v"(key_at), "+v"(value_at));
@@ -713,13 +808,13 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
             add_values<IO, KV, D, 1>(v, w, g, s);
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's LDS
     if (bad && a.status) atomicOr(a.status, bad);
     s.l[0] += __shfl_xor(s.l[0], 16, kWave);
     s.l[0] += __shfl_xor(s.l[0], 32, kWave);
+    const size_t tile = (((size_t)kvh * c.chunks + at_piece.chunk) * c.blocks + at_piece.block) * kManyWaves + wave;
     if (mine < queries)
-        store_sums<W, D>(c.prefix_stats, c.prefix_o,
-                         ((size_t)(kvh * c.chunks + at_piece.chunk) * c.blocks) * kManyQueries + mine, s.o[0], s.ref[0],
-                         s.l[0], quarter);
+        store_sums<D>(c.prefix_stats + tile * 16, c.prefix_o + tile * 16 * D, 16, col, s.o[0], s.ref[0], s.l[0], quarter);
 }
 
 template <bool IO, bool KV, int D>
@@ -730,62 +825,97 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_attn_many_kernel(Pag
     else own_block<IO, KV, D, kManyWaves>(a, c, blockIdx.x - over_prefix, lds);
 }
 
-// Workgroup (query head, row, 64 elements): 16 lanes hold the elements, the
-// 16 lane groups of the four waves join pieces g, g + 16, ... in order, the
-// prefix's first, then the groups are added in order.  Every wave reads all
-// pieces' m and l itself, so nothing waits for a barrier before the sums.
-template <bool IO, int D>
+// Workgroup (kv head, row, four accumulators): a thread owns 16 bytes of the
+// pieces, (accumulator, quarter, query), and every n-th piece; the n threads
+// of one item are joined at the end, in order.
+template <bool IO, int D, int W>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c) {
-    __shared__ v4f parts[16][16];
-    const uint32_t h = blockIdx.x, r = blockIdx.y;
-    const int tid = threadIdx.x, lane = tid & 63;
-    const uint32_t kvs = a.pool.kv_heads, kvh = h / a.group, in_group = h - kvh * a.group;
-    const uint2 run = c.runs[r * kvs + kvh];  // first wave, pieces
+    __shared__ v4f parts[256];
+    __shared__ float2 stats[256];
+    const uint32_t kvh = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+    const Run run = c.runs[r * a.pool.kv_heads + kvh];
+    const uint32_t items = 16 * a.group, n = 256 / items, item = tid % items, nth = tid / items;
+    const uint32_t col = item % a.group, fq = blockIdx.z * 16 + item / a.group;
+    const uint32_t chunks = c.chunks, pieces = chunks + run.heads + run.mids + run.tails;
     if (a.lengths[r] < 0) return;
-    const uint32_t chunks = c.chunks, pieces = chunks + run.y;
-    const size_t prefix_at = (size_t)kvh * c.chunks * c.blocks * c.block + r * a.group + in_group;
-    const size_t prefix_step = (size_t)c.blocks * c.block;
-    const size_t own_at = ((size_t)run.x + r * kvs + kvh) * a.group + in_group;
-    const int e = blockIdx.z * 64 + 4 * (tid & 15), g = tid >> 4;
-    auto stats = [&](uint32_t i) {
-        return i < chunks ? c.prefix_stats[prefix_at + i * prefix_step] : c.own_stats[own_at + (size_t)(i - chunks) * a.group];
-    };
-    auto elements = [&](uint32_t i) {
-        return *(const v4f*)((i < chunks ? c.prefix_o + (prefix_at + i * prefix_step) * D
-                                         : c.own_o + (own_at + (size_t)(i - chunks) * a.group) * D) + e);
-    };
+    const uint32_t query = r * a.group + col;
+    const size_t tiles = (size_t)c.blocks * c.block / 16;  // of 16 queries, per piece of the prefix
+    const size_t prefix_tile = kvh * chunks * tiles + query / 16, own_base = r * a.pool.kv_heads + kvh;
+    const float2* stat[kJoin];
+    const float* from[kJoin];
     float top = -INFINITY, l = 0.0f;
     v4f o = {};
-    // 64 pieces at a time, the sums brought to the highest m so far
-    for (uint32_t from = 0; from < pieces; from += 64) {
-        const uint32_t n = min(64u, pieces - from);
-        // this lane's piece of the 64, and the lane group's four
-        const float2 x = (uint32_t)lane < n ? stats(from + lane) : make_float2(-INFINITY, 0.0f);
-        v4f p[4];
+    if (nth < n)
+        for (uint32_t i = nth; i < pieces; i += kJoin * n) {
+            v4f x[kJoin];
+            float2 y[kJoin];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (g + 16 * u < n) p[u] = elements(from + g + 16 * u);
-        const float to = fmaxf(top, wave_max(x.x)), sub = to == -INFINITY ? 0.0f : to;
-        const float keep = __builtin_amdgcn_exp2f(top == to ? 0.0f : top - sub);
-        const float w = __builtin_amdgcn_exp2f(x.x == to ? 0.0f : x.x - sub);
-        l = l * keep + wave_sum_xor((uint32_t)lane < n ? w * x.y : 0.0f, kWave);
-        o *= keep;
+            for (int u = 0; u < kJoin; ++u) {
+                // past the last piece: the last one, with no weight
+                const uint32_t p = min(i + u * n, pieces - 1);
+                if (p < chunks) {
+                    const size_t tile = prefix_tile + p * tiles;
+                    stat[u] = c.prefix_stats + tile * 16 + query % 16;
+                    from[u] = c.prefix_o + (tile * 16 * D + (fq * 16 + query % 16) * 4);
+                } else {
+                    uint32_t w = p - chunks;
+                    if (w < run.heads) w += run.head;
+                    else if (w < run.heads + run.mids) w = run.mid + (w - run.heads) * run.active;
+                    else w = run.tail + (w - run.heads - run.mids);
+                    const size_t piece = own_base + w;
+                    stat[u] = c.own_stats + piece * a.group + col;
+                    from[u] = c.own_o + (piece * a.group * D + (fq * a.group + col) * 4);
+                }
+                y[u] = *stat[u];
+                x[u] = *(const v4f*)from[u];
+            }
+            float to = top;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float wu = __shfl(w, g + 16 * u, kWave);
-            if (g + 16 * u < n) o += wu * p[u];
+            for (int u = 0; u < kJoin; ++u) to = fmaxf(to, y[u].x);
+            const float sub = to == -INFINITY ? 0.0f : to;
+            const float keep = __builtin_amdgcn_exp2f(top == to ? 0.0f : top - sub);
+            l *= keep;
+            o *= keep;
+            top = to;
+#pragma unroll
+            for (int u = 0; u < kJoin; ++u)
+                if (i + u * n < pieces) {
+                    const float e = __builtin_amdgcn_exp2f(y[u].x == to ? 0.0f : y[u].x - sub);
+                    l += e * y[u].y;
+                    o += e * x[u];
+                }
         }
-        top = to;
-    }
-    parts[g][tid & 15] = o;
+    parts[tid] = o;
+    stats[tid] = make_float2(top, l);
     __syncthreads();
-    if (tid >= 16) return;
-    o = parts[0][tid];
+    if (tid < items) {
+        float to = top;
+        for (uint32_t i = 1; i < n; ++i) to = fmaxf(to, stats[tid + i * items].x);
+        const float sub = to == -INFINITY ? 0.0f : to;
+        const float keep = __builtin_amdgcn_exp2f(top == to ? 0.0f : top - sub);
+        l *= keep;
+        o *= keep;
+        for (uint32_t i = 1; i < n; ++i) {
+            const float2 y = stats[tid + i * items];
+            const float e = __builtin_amdgcn_exp2f(y.x == to ? 0.0f : y.x - sub);
+            l += e * y.y;
+            o += e * parts[tid + i * items];
+        }
 #pragma unroll
-    for (int i = 1; i < 16; ++i) o += parts[i][tid];
+        for (int j = 0; j < 4; ++j) o[j] = l == 0.0f ? 0.0f : o[j] / l;
+    }
+    __syncthreads();
+    if (tid < items) parts[tid] = o;
+    __syncthreads();
+    // accumulators 4 z .. 4 z + 3 are four successive elements: thread (query,
+    // quarter, register) stores them
+    if (tid >= items) return;
+    const uint32_t head = tid / 16, quarter = tid / 4 % 4, reg = tid % 4, f = blockIdx.z * 4;
+    v4f out;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = l == 0.0f ? 0.0f : o[j] / l;
-    store4<IO>(a.out, r * a.out_stride + (size_t)h * D + e, o);
+    for (int j = 0; j < 4; ++j) out[j] = parts[(j * 4 + quarter) * a.group + head][reg];
+    store4<IO>(a.out, r * a.out_stride + (size_t)(kvh * a.group + head) * D + 16 * W * (f / W) + W * (4 * quarter + reg) + f % W,
+               out);
 }
 
 // ------------------------------------------------------------------- host
@@ -815,16 +945,16 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
     const bool many = c.chunks && c.block == kManyQueries;
     c.per_group = many && kManyWaves * group * query_bytes <= kOwnLds ? kManyWaves : 4;
     const uint64_t own_tiles = (uint64_t)rows * kv_heads * ((row_tokens + tile - 1) / tile);
-    c.waves = c.per_group * (int)std::min<uint64_t>(kOwnWaves / c.per_group, own_tiles);
+    c.groups = (int)std::min<uint64_t>(kOwnWaves / c.per_group, own_tiles);
     const size_t prefix_rows = (size_t)kv_heads * c.chunks * c.blocks * c.block;
-    const size_t own_rows = ((size_t)c.waves + (size_t)rows * kv_heads) * group;
+    const size_t own_rows = ((size_t)c.groups * c.per_group + (size_t)rows * kv_heads) * group;
     char* at = (char*)workspace;
     auto take = [&](size_t n) {
         char* p = at;
         at += (n + 255) / 256 * 256;
         return p;
     };
-    c.runs = (uint2*)take((size_t)rows * kv_heads * sizeof(uint2));
+    c.runs = (Run*)take((size_t)rows * kv_heads * sizeof(Run));
     c.prefix_stats = (float2*)take(prefix_rows * sizeof(float2));
     c.own_stats = (float2*)take(own_rows * sizeof(float2));
     c.prefix_o = (float*)take(prefix_rows * head_dim * sizeof(float));
@@ -855,10 +985,10 @@ static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
     const bool many = c.chunks && c.block == kManyQueries;
     const int waves = many ? kManyWaves : 4;
     constexpr size_t query = query_bytes<IO, KV, D>();
-    const size_t own = table_bytes(a.rows, waves) + c.per_group * a.group * query;
+    const size_t own = std::max(table_bytes(a.rows, waves) + c.per_group * a.group * query, gather_bytes(c.per_group, 1, D));
     size_t prefix = 0;
-    if (many) prefix = (size_t)4 * F::kTile * D * (KV ? 2 : 4);  // two tiles' keys and values
-    else if (c.chunks) prefix = std::max(query * c.block, (size_t)4 * c.block * 8 + (size_t)2 * c.block * D * 4);
+    if (many) prefix = (size_t)kBuffers * 2 * F::kTile * D * (KV ? 2 : 4) + (size_t)kSegment * F::kTile * 4;
+    else if (c.chunks) prefix = std::max(query * c.block, gather_bytes(4, c.block / 16, D));
     const size_t lds = std::max(prefix, own);
     void (*kernel)(PagedAttnArgs, Cut) = many                            ? paged_attn_many_kernel<IO, KV, D>
                                          : c.chunks && c.block == 32 ? paged_attn_kernel<IO, KV, D, 2>
@@ -867,10 +997,10 @@ static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
         hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    kernel<<<c.chunks * c.blocks * a.pool.kv_heads + c.waves / c.per_group, 64 * waves, lds, st>>>(a, c);
+    kernel<<<c.chunks * c.blocks * a.pool.kv_heads + c.groups, 64 * waves, lds, st>>>(a, c);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    paged_join_kernel<IO, D><<<dim3(a.q_heads, a.rows, D / 64), 256, 0, st>>>(a, c);
+    paged_join_kernel<IO, D, F::kWide><<<dim3(a.pool.kv_heads, a.rows, D / 64), 256, 0, st>>>(a, c);
     return hipGetLastError();
 }
 
