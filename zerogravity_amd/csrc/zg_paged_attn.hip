@@ -32,7 +32,9 @@ constexpr int kOwnWaves = 2048;     // waves over the rows' own tiles: two per S
 constexpr int kManyTiles = 2;       // fewest tiles of a piece of the prefix for 128 queries
 constexpr int kPrefixGroups = 256;  // about so many over the prefix
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
+constexpr int kCus = 256;
 constexpr int kJoin = 8;             // pieces that a thread of the join has under way
+constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRaise = 8.0f;      // log2: how far a score may pass the reference before sums are rescaled
 
 template <bool IO, bool KV, int D>
@@ -42,6 +44,9 @@ struct Form {
     // parts of a weight: 2^-16 of it is left out, a 256th of the output's
     // own rounding.
     static constexpr int kParts = KV ? (IO ? 1 : 3) : 1;
+    // the scale (in log2) is put on the queries, but for those that enter as
+    // the bfloat16 they are
+    static constexpr bool kScaled = !(KV && IO);
     static constexpr int kWeightParts = KV ? (IO ? 2 : 3) : 1;
     static constexpr int kSteps = KV ? D / 32 : D / 16;                // 16 bytes of a key per lane and step
     static constexpr int kWide = KV ? (D / 16 < 8 ? D / 16 : 8) : 4;   // elements of a value row per lane and load
@@ -65,18 +70,18 @@ __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
 // Queries in LDS in operand order, 16 bytes per (step, part, quarter, query):
 // a wave's read is contiguous.  `who` gives query m's elements in memory.
 template <bool IO, bool KV, int D, typename Who>
-__device__ __forceinline__ void stage_queries(v4u* lds, int n, int thread, int threads, Who who) {
+__device__ __forceinline__ void stage_queries(v4u* lds, int n, int thread, int threads, float to_log2, Who who) {
     using F = Form<IO, KV, D>;
     constexpr int E = KV ? 8 : 4;
     for (int i = thread; i < n * (D / E); i += threads) {
         const int m = i % n, c = i / n;
         const size_t at = who(m) + c * E;
         if constexpr (!KV) {
-            lds[c * n + m] = __builtin_bit_cast(v4u, load4<IO>(who.base, at));
+            lds[c * n + m] = __builtin_bit_cast(v4u, load4<IO>(who.base, at) * to_log2);
         } else if constexpr (IO) {
             lds[c * n + m] = *(const v4u*)((const uint16_t*)who.base + at);
         } else {
-            v4f x[2] = {load4<false>(who.base, at), load4<false>(who.base, at + 4)};
+            v4f x[2] = {load4<false>(who.base, at) * to_log2, load4<false>(who.base, at + 4) * to_log2};
 #pragma unroll
             for (int p = 0; p < F::kParts; ++p) {
                 v4u w;
@@ -128,25 +133,65 @@ __device__ __forceinline__ Place resolve(const PagedPool& p, uint32_t page, uint
     return at;
 }
 
+// A tile's weights as operands of the second product.
+template <bool IO, bool KV, int D, int MT>
+struct Weights {
+    static constexpr int kParts = Form<IO, KV, D>::kWeightParts, kMine = Form<IO, KV, D>::kMine;
+    v4u part[MT][kParts];  // of bfloat16; a 32-bit cache takes the weights as they are
+    __device__ void operator=(const float (&w)[MT][kMine]) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if constexpr (!KV) {
+                part[m][0] = v4u{__float_as_uint(w[m][0]), __float_as_uint(w[m][1]), __float_as_uint(w[m][2]),
+                                 __float_as_uint(w[m][3])};
+            } else {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = w[m][j];
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) part[m][p][j] = pack_high(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] -= high_part(x[j]);
+                }
+            }
+        }
+    }
+};
+
+// The value of the lane 16 or 32 further on (xor), without the LDS.
+template <int XOR>
+__device__ __forceinline__ float other_quarter(float x) {
+    if constexpr (XOR == 16) {
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+        return __int_as_float((threadIdx.x & 16) ? y[0] : y[1]);
+    } else {
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+        return __int_as_float((threadIdx.x & 32) ? y[0] : y[1]);
+    }
+}
+
 // A tile's weights e^(s - m) from its scores, m the query's reference: the
 // sums are brought to a new one only when a score passes the old one by
 // 2^kRaise, which 32-bit sums hold with ease.
 template <bool IO, bool KV, int D, int MT>
 __device__ __forceinline__ void weigh(const v4f (&sc)[MT][Form<IO, KV, D>::kHalves], uint32_t there, float to_log2,
-                                      int quarter, Sums<D, MT>& s, float (&w)[MT][Form<IO, KV, D>::kMine]) {
+                                      int quarter, Sums<D, MT>& s, Weights<IO, KV, D, MT>& weights) {
     constexpr int N = Form<IO, KV, D>::kMine;
+    float w[MT][N];
     constexpr uint32_t kAll = N == 8 ? 0xffffffffu : 0xffffu;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            w[m][j] = sc[m][j >> 2][j & 3] * to_log2;
+            w[m][j] = Form<IO, KV, D>::kScaled ? sc[m][j >> 2][j & 3] : sc[m][j >> 2][j & 3] * to_log2;
             if (there != kAll && !(there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u)) w[m][j] = -INFINITY;
             top = fmaxf(top, w[m][j]);
         }
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = fmaxf(top, other_quarter<16>(top));
+        top = fmaxf(top, other_quarter<32>(top));
         if (__any(top > s.ref[m] + kRaise)) {
             const float to = fmaxf(top, s.ref[m]);
             const float keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.ref[m] - to);
@@ -162,6 +207,7 @@ __device__ __forceinline__ void weigh(const v4f (&sc)[MT][Form<IO, KV, D>::kHalv
             s.l[m] += w[m][j];
         }
     }
+    weights = w;
 }
 
 // Values of tokens that are not there weigh 0, and may be anything.
@@ -178,24 +224,11 @@ __device__ __forceinline__ void drop_values(uint32_t (&v)[N][VR], uint32_t there
 
 // One load's worth of a tile's value rows, weighted, added to the sums.
 template <bool IO, bool KV, int D, int MT, int N, int VR>
-__device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const float (&w)[MT][N], int g, Sums<D, MT>& s) {
+__device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const Weights<IO, KV, D, MT>& w, int g,
+                                           Sums<D, MT>& s) {
     using F = Form<IO, KV, D>;
     constexpr int W = F::kWide;
     if constexpr (KV) {
-        v4u part[MT][F::kWeightParts];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = w[m][j];
-#pragma unroll
-            for (int p = 0; p < F::kWeightParts; ++p) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part[m][p][j] = pack_high(x[2 * j], x[2 * j + 1]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] -= high_part(x[j]);
-            }
-        }
         // two accumulators at a time: a product waits for the one before it on
         // the same accumulator (four would not leave the registers for it)
 #pragma unroll
@@ -213,7 +246,7 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const flo
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
-                        s.o[m][g * W + from + i] = mfma_bf16(rows[i], part[m][p], s.o[m][g * W + from + i]);
+                        s.o[m][g * W + from + i] = mfma_bf16(rows[i], w.part[m][p], s.o[m][g * W + from + i]);
         }
     } else {
 #pragma unroll
@@ -222,8 +255,8 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const flo
             for (int i = 0; i < W; ++i)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
-                    s.o[m][g * W + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][i]), w[m][j],
-                                                                             s.o[m][g * W + i], 0, 0, 0);
+                    s.o[m][g * W + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        __uint_as_float(v[j][i]), __uint_as_float(w.part[m][0][j]), s.o[m][g * W + i], 0, 0, 0);
     }
 }
 
@@ -236,7 +269,7 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
     constexpr int W = F::kWide, H = F::kHalves, N = F::kMine;
     constexpr int ES = KV ? 2 : 4, VR = W * ES / 4;  // registers of a value row per load
     const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
-    const float to_log2 = a.scale * 1.44269504088896341f;
+    const float to_log2 = F::kScaled ? 1.0f : a.scale * kLog2e;
     const char* const keys = (const char*)a.pool.keys;
     const char* const values = (const char*)a.pool.values;
     constexpr uint32_t kAll = H == 2 ? 0xffffffffu : 0xffffu;
@@ -316,7 +349,7 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
 #pragma unroll
         for (int g = kFirst; g < F::kLoads; ++g) load_values(g);
         __builtin_amdgcn_sched_barrier(0);
-        float w[MT][N];
+        Weights<IO, KV, D, MT> w;
         weigh<IO, KV, D, MT>(sc, there, to_log2, quarter, s, w);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -444,6 +477,17 @@ __device__ __forceinline__ uint32_t own_tokens(const PagedAttnArgs& a, uint32_t 
     const int n = a.lengths[r];
     return n < 0 ? 0 : min((uint32_t)n, a.stride * a.pool.page_tokens.d);
 }
+// A query's triple of one piece of the prefix; the pieces lie like the rows'
+// own, one after the other for all rows.
+template <int D>
+__device__ __forceinline__ void store_prefix(const PagedAttnArgs& a, const Cut& c, int piece, int query,
+                                             const v4f (&from)[D / 16], float ref, float l, int quarter) {
+    const int row = query / a.group;
+    if (row >= (int)a.rows) return;
+    const size_t at = ((size_t)piece * a.rows + row) * a.group;
+    store_sums<D>(c.prefix_stats + at, c.prefix_o + at * D, a.group, query - row * a.group, from, ref, l, quarter);
+}
+
 // The piece of the prefix that a workgroup takes.  Workgroups id, id + 8, id +
 // 16, ... run on one XCD: they are given the blocks of one piece, which that
 // L2 then reads from memory once.
@@ -482,7 +526,7 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
             return r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
         }
     } who{a.q, a, block * 16 * MT, queries - 1, kvh};
-    stage_queries<IO, KV, D>((v4u*)lds, 16 * MT, tid, 256, who);
+    stage_queries<IO, KV, D>((v4u*)lds, 16 * MT, tid, 256, a.scale * kLog2e, who);
     __syncthreads();
     Sums<D, MT> s;
     s.clear();
@@ -494,12 +538,9 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
     __syncthreads();
     gather_waves<D, MT>(s, 4, wave, lane, lds);
     if (wave) return;
-    const size_t tile = (((size_t)kvh * c.chunks + chunk) * c.blocks + block) * MT;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
-        if (block * 16 * MT + 16 * m + col < queries)
-            store_sums<D>(c.prefix_stats + (tile + m) * 16, c.prefix_o + (tile + m) * 16 * D, 16, col, s.o[m], s.ref[m],
-                          s.l[m], quarter);
+        store_prefix<D>(a, c, kvh * c.chunks + chunk, block * 16 * MT + 16 * m + col, s.o[m], s.ref[m], s.l[m], quarter);
 }
 
 // What a wave wrote to LDS, its other lanes read after this.
@@ -607,7 +648,7 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
             size_t first;
             __device__ size_t operator()(int m) const { return first + (size_t)m * D; }
         } who{a.q, r * a.q_stride + (size_t)kvh * a.group * D};
-        stage_queries<IO, KV, D>(queries, a.group, lane, 64, who);
+        stage_queries<IO, KV, D>(queries, a.group, lane, 64, a.scale * kLog2e, who);
         same_wave();
         add_tiles<IO, KV, D, 1>(a, queries, a.group, a.table + (size_t)r * a.stride, own_tokens(a, r), (int)tile,
                                 (int)upto_tile, 1, (int)kvh, s, bad);
@@ -643,7 +684,7 @@ __global__ __launch_bounds__(256, MT * D > 256 ? 1 : 2) void paged_attn_kernel(P
 }
 
 constexpr int kManyWaves = 8, kManyQueries = 16 * kManyWaves;
-constexpr int kBuffers = 4, kAhead = kBuffers - 1;  // tiles in LDS, and copied ahead of the one in use
+constexpr int kBuffers = 4;                         // tiles in LDS: two in use, two coming
 constexpr int kSegment = 64;                        // tiles looked up at a time
 
 // Many queries over the prefix: each of eight waves holds 16 queries and their
@@ -662,7 +703,7 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
     constexpr uint32_t kAll = H == 2 ? 0xffffffffu : 0xffffu;
     const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const float to_log2 = a.scale * 1.44269504088896341f;
+    const float to_log2 = F::kScaled ? 1.0f : a.scale * kLog2e;
     const PieceOf at_piece = piece_of(c, a.pool.kv_heads, id);
     const int kvh = at_piece.kvh, queries = (int)a.rows * a.group;
     const int first = at_piece.chunk * c.chunk_tiles, end = min(first + c.chunk_tiles, c.prefix_tiles);
@@ -672,6 +713,23 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
     int key_at = col * kRow + 16 * (quarter ^ swizzle(col));
     int value_at = kHalf + 4 * quarter * kRow +
                    (VR == 4 ? 16 * (col ^ swizzle(4 * quarter)) : 16 * ((col >> 1) ^ swizzle(4 * quarter)) + 8 * (col & 1));
+
+    // the wave's queries: asked for first, used last
+    const int mine = at_piece.block * kManyQueries + 16 * wave + col, f = min(mine, queries - 1), r = f / a.group;
+    const size_t from = r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
+    const bool live = at_piece.block * kManyQueries + 16 * wave < queries;
+    v4u raw[F::kSteps][KV && !IO ? 2 : 1];
+#pragma unroll
+    for (int i = 0; i < F::kSteps; ++i) {
+        if constexpr (!KV) {
+            raw[i][0] = __builtin_bit_cast(v4u, load4<IO>(a.q, from + 16 * i + 4 * quarter));
+        } else if constexpr (IO) {
+            raw[i][0] = *(const v4u*)((const uint16_t*)a.q + from + 32 * i + 8 * quarter);
+        } else {
+            raw[i][0] = *(const v4u*)((const float*)a.q + from + 32 * i + 8 * quarter);
+            raw[i][1] = *(const v4u*)((const float*)a.q + from + 32 * i + 8 * quarter + 4);
+        }
+    }
 
     // the places of a segment's tokens, looked up once for the workgroup; all
     // ones: the token is not there
@@ -709,25 +767,33 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
             units[i] = unit;
         }
     };
+    // the copies of tiles `local` and the next, and which of their tokens are
+    // there; past the segment's last tile that one again
     int held = min(kSegment, end - first);  // tiles of the segment in `units`
+    uint32_t coming[2];
+    auto fetch = [&](int local, int buffer) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = min(local + i, held - 1);
+            coming[i] = (uint32_t)__ballot(units[x * F::kTile + (lane & (F::kTile - 1))] != ~0u) & kAll;
+            copy(x, buffer + i);
+        }
+    };
     look_up(first, held);
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) copy(min(i, held - 1), i);
+    fetch(0, 0);
 
-    // the wave's queries, in operand order
-    const int mine = at_piece.block * kManyQueries + 16 * wave + col, f = min(mine, queries - 1), r = f / a.group;
-    const size_t from = r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
-    const bool live = at_piece.block * kManyQueries + 16 * wave < queries;
+    // the queries' parts, in operand order
     v4u q[F::kParts][F::kSteps];
 #pragma unroll
     for (int i = 0; i < F::kSteps; ++i) {
         if constexpr (!KV) {
-            q[0][i] = __builtin_bit_cast(v4u, load4<IO>(a.q, from + 16 * i + 4 * quarter));
+            q[0][i] = __builtin_bit_cast(v4u, __builtin_bit_cast(v4f, raw[i][0]) * (a.scale * kLog2e));
         } else if constexpr (IO) {
-            q[0][i] = *(const v4u*)((const uint16_t*)a.q + from + 32 * i + 8 * quarter);
+            q[0][i] = raw[i][0];
         } else {
-            v4f x[2] = {load4<false>(a.q, from + 32 * i + 8 * quarter), load4<false>(a.q, from + 32 * i + 8 * quarter + 4)};
+            v4f x[2] = {__builtin_bit_cast(v4f, raw[i][0]) * (a.scale * kLog2e),
+                        __builtin_bit_cast(v4f, raw[i][1]) * (a.scale * kLog2e)};
 #pragma unroll
             for (int p = 0; p < F::kParts; ++p) {
 #pragma unroll
@@ -739,8 +805,39 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
     }
     Sums<D, 1> s;
     s.clear();
-    for (int tile = first, local = 0; tile < end; ++tile, ++local) {
-        if (local == held) {
+    Weights<IO, KV, D, 1> w;
+    uint32_t v[N][VR];
+    auto load_values = [&](int g, int buffer) {
+        const char* const data = lds + buffer * 2 * kHalf;
+        if (g == 0) asm volatile("" : "+v"(value_at));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int exchange = 16 * (kPieces >= 16 ? j & 3 : (j & 3) >> 1);
+            const char* from = data + (value_at ^ exchange) + (16 * (j >> 2) + (j & 3)) * kRow + 256 * g;
+            if constexpr (VR == 4) {
+                const v4u x = *(const v4u*)from;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[j][y] = x[y];
+            } else {
+                const uint2 x = *(const uint2*)from;
+                v[j][0] = x.x;
+                v[j][1] = x.y;
+            }
+        }
+    };
+    // a tile's values, the first load of them on its way already
+    auto add = [&](uint32_t there, int buffer) {
+#pragma unroll
+        for (int g = 0; g < F::kLoads; ++g) {
+            if (g) load_values(g, buffer);
+            drop_values<KV>(v, there, quarter);
+            add_values<IO, KV, D, 1>(v, w, g, s);
+        }
+    };
+    // Two tiles between barriers: within them the two waves of a SIMD drift
+    // apart, so that one's products run beside the other's weights.
+    for (int tile = first, local = 0; tile < end; tile += 2, local += 2) {
+        if (local >= held) {
             // the next segment: everyone is done with this one, and the copies
             // past its end have landed
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -748,81 +845,81 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
             held = min(kSegment, end - tile);
             look_up(tile, held);
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) copy(min(i, held - 1), i);
             local = 0;
+            fetch(0, (tile - first) & 2);
         }
-        const uint32_t there = (uint32_t)__ballot(units[local * F::kTile + (lane & (F::kTile - 1))] != ~0u) & kAll;
-        const int buffer = local % kBuffers;
-        // this tile's copies have landed when no more are under way than the
-        // later tiles'; after the barrier everyone's have, and the buffer of
-        // the tile before has been read
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kAhead - 1) * kCopies) : "memory");
-        // past the segment's last tile that one again, so that the count holds
-        copy(min(local + kAhead, held - 1), (buffer + kAhead) % kBuffers);
-        if (!live) continue;
+        uint32_t there[2] = {coming[0], coming[1]};
+        const int pair = (tile - first) & 2;  // its first buffer
+        // both tiles' copies have landed; after the barrier everyone's have,
+        // and the other two buffers have been read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (!live) {
+            fetch(local + 2, pair ^ 2);
+            continue;
+        }
+#pragma unroll 1
+        for (int half = 0; half < 2 && tile + half < end; ++half) {
+        const int buffer = pair + half;
         const char* const data = lds + buffer * 2 * kHalf;
-        asm volatile("" : "+v"(key_at), "+v"(value_at));
-        v4f sc[H];
+        asm volatile("" : "+v"(key_at));
+        // the keys of two steps are on their way while a third is used
+        v4u k[3][H];
+        auto load_keys = [&](int i) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) sc[h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int h = 0; h < H; ++h)
+                k[i % 3][h] = *(const v4u*)(data + (key_at ^ 64 * (i & 3)) + 16 * h * kRow + 256 * (i / 4));
+        };
+        load_keys(0);
+        if (F::kSteps > 1) load_keys(1);
+        v4f sc[1][H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) sc[0][h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < F::kSteps; ++i) {
-            v4u k[H];
-#pragma unroll
-            for (int h = 0; h < H; ++h) k[h] = *(const v4u*)(data + (key_at ^ 64 * (i & 3)) + 16 * h * kRow + 256 * (i / 4));
+            if (i + 2 < F::kSteps) load_keys(i + 2);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int p = 0; p < F::kParts; ++p)
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     if constexpr (KV) {
-                        sc[h] = mfma_bf16(k[h], q[p][i], sc[h]);
+                        sc[0][h] = mfma_bf16(k[i % 3][h], q[p][i], sc[0][h]);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h][e]),
-                                                                         __uint_as_float(q[0][i][e]), sc[h], 0, 0, 0);
+                            sc[0][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i % 3][h][e]),
+                                                                            __uint_as_float(q[0][i][e]), sc[0][h], 0, 0, 0);
                     }
                 }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        float w[1][N];
-        weigh<IO, KV, D, 1>((const v4f(&)[1][H])sc, there, to_log2, quarter, s, w);
-#pragma unroll
-        for (int g = 0; g < F::kLoads; ++g) {
-            uint32_t v[N][VR];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int exchange = 16 * (kPieces >= 16 ? j & 3 : (j & 3) >> 1);
-                const char* from = data + (value_at ^ exchange) + (16 * (j >> 2) + (j & 3)) * kRow + 256 * g;
-                if constexpr (VR == 4) {
-                    const v4u x = *(const v4u*)from;
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) v[j][y] = x[y];
-                } else {
-                    const uint2 x = *(const uint2*)from;
-                    v[j][0] = x.x;
-                    v[j][1] = x.y;
-                }
-            }
-            drop_values<KV>(v, there, quarter);
-            add_values<IO, KV, D, 1>(v, w, g, s);
+        load_values(0, buffer);
+        if (half == 0) fetch(local + 2, pair ^ 2);
+        __builtin_amdgcn_sched_barrier(0);
+        weigh<IO, KV, D, 1>(sc, there[half], to_log2, quarter, s, w);
+        add(there[half], buffer);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's LDS
     if (bad && a.status) atomicOr(a.status, bad);
     s.l[0] += __shfl_xor(s.l[0], 16, kWave);
     s.l[0] += __shfl_xor(s.l[0], 32, kWave);
-    const size_t tile = (((size_t)kvh * c.chunks + at_piece.chunk) * c.blocks + at_piece.block) * kManyWaves + wave;
-    if (mine < queries)
-        store_sums<D>(c.prefix_stats + tile * 16, c.prefix_o + tile * 16 * D, 16, col, s.o[0], s.ref[0], s.l[0], quarter);
+    store_prefix<D>(a, c, kvh * c.chunks + at_piece.chunk, mine, s.o[0], s.ref[0], s.l[0], quarter);
 }
 
 template <bool IO, bool KV, int D>
 __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_attn_many_kernel(PagedAttnArgs a, Cut c) {
     extern __shared__ __align__(16) char lds[];
-    const int over_prefix = c.chunks * c.blocks * a.pool.kv_heads;
-    if ((int)blockIdx.x < over_prefix) many_block<IO, KV, D>(a, c, blockIdx.x, lds);
-    else own_block<IO, KV, D, kManyWaves>(a, c, blockIdx.x - over_prefix, lds);
+    // One workgroup fits a CU: those that take a piece of the prefix are the
+    // first, the rows' own tiles go to the last ones, and where they meet a
+    // workgroup does one after the other.
+    const int over_prefix = c.chunks * c.blocks * a.pool.kv_heads, own = (int)gridDim.x - 1 - (int)blockIdx.x;
+    if ((int)blockIdx.x < over_prefix) {
+        many_block<IO, KV, D>(a, c, blockIdx.x, lds);
+        if (own >= c.groups) return;
+        __syncthreads();
+    }
+    if (own < c.groups) own_block<IO, KV, D, kManyWaves>(a, c, own, lds);
 }
 
 // Workgroup (kv head, row, four accumulators): a thread owns 16 bytes of the
@@ -838,11 +935,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c)
     const uint32_t col = item % a.group, fq = blockIdx.z * 16 + item / a.group;
     const uint32_t chunks = c.chunks, pieces = chunks + run.heads + run.mids + run.tails;
     if (a.lengths[r] < 0) return;
-    const uint32_t query = r * a.group + col;
-    const size_t tiles = (size_t)c.blocks * c.block / 16;  // of 16 queries, per piece of the prefix
-    const size_t prefix_tile = kvh * chunks * tiles + query / 16, own_base = r * a.pool.kv_heads + kvh;
-    const float2* stat[kJoin];
-    const float* from[kJoin];
+    const size_t own_base = r * a.pool.kv_heads + kvh;
     float top = -INFINITY, l = 0.0f;
     v4f o = {};
     if (nth < n)
@@ -853,21 +946,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c)
             for (int u = 0; u < kJoin; ++u) {
                 // past the last piece: the last one, with no weight
                 const uint32_t p = min(i + u * n, pieces - 1);
-                if (p < chunks) {
-                    const size_t tile = prefix_tile + p * tiles;
-                    stat[u] = c.prefix_stats + tile * 16 + query % 16;
-                    from[u] = c.prefix_o + (tile * 16 * D + (fq * 16 + query % 16) * 4);
-                } else {
-                    uint32_t w = p - chunks;
-                    if (w < run.heads) w += run.head;
-                    else if (w < run.heads + run.mids) w = run.mid + (w - run.heads) * run.active;
-                    else w = run.tail + (w - run.heads - run.mids);
-                    const size_t piece = own_base + w;
-                    stat[u] = c.own_stats + piece * a.group + col;
-                    from[u] = c.own_o + (piece * a.group * D + (fq * a.group + col) * 4);
-                }
-                y[u] = *stat[u];
-                x[u] = *(const v4f*)from[u];
+                uint32_t w = p - chunks;
+                if (w < run.heads) w += run.head;
+                else if (w < run.heads + run.mids) w = run.mid + (w - run.heads) * run.active;
+                else w = run.tail + (w - run.heads - run.mids);
+                const bool shared = p < chunks;
+                const size_t at = (shared ? (size_t)(kvh * chunks + p) * a.rows + r : own_base + w) * a.group;
+                y[u] = (shared ? c.prefix_stats : c.own_stats)[at + col];
+                x[u] = *(const v4f*)((shared ? c.prefix_o : c.own_o) + at * D + (fq * a.group + col) * 4);
             }
             float to = top;
 #pragma unroll
@@ -945,8 +1031,14 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
     const bool many = c.chunks && c.block == kManyQueries;
     c.per_group = many && kManyWaves * group * query_bytes <= kOwnLds ? kManyWaves : 4;
     const uint64_t own_tiles = (uint64_t)rows * kv_heads * ((row_tokens + tile - 1) / tile);
-    c.groups = (int)std::min<uint64_t>(kOwnWaves / c.per_group, own_tiles);
-    const size_t prefix_rows = (size_t)kv_heads * c.chunks * c.blocks * c.block;
+    int most = kOwnWaves / c.per_group;
+    if (many) {
+        // the CUs that the prefix leaves, if they are a quarter of them
+        const int left = kCus - c.chunks * c.blocks * kv_heads;
+        most = left >= kCus / 4 ? left : kCus;
+    }
+    c.groups = (int)std::min<uint64_t>(most, own_tiles);
+    const size_t prefix_rows = (size_t)kv_heads * c.chunks * rows * group;
     const size_t own_rows = ((size_t)c.groups * c.per_group + (size_t)rows * kv_heads) * group;
     char* at = (char*)workspace;
     auto take = [&](size_t n) {
@@ -997,7 +1089,8 @@ static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
         hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    kernel<<<c.chunks * c.blocks * a.pool.kv_heads + c.groups, 64 * waves, lds, st>>>(a, c);
+    const int over_prefix = c.chunks * c.blocks * a.pool.kv_heads;
+    kernel<<<many ? std::max(over_prefix, kCus) : over_prefix + c.groups, 64 * waves, lds, st>>>(a, c);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     paged_join_kernel<IO, D, F::kWide><<<dim3(a.pool.kv_heads, a.rows, D / 64), 256, 0, st>>>(a, c);
