@@ -21,6 +21,7 @@
 // So the tile needs neither LDS nor a barrier, and each key and value is read
 // from memory once per 16 MT queries.
 #include <algorithm>
+#include <cmath>
 
 #include "zg_paged.hpp"
 
@@ -29,8 +30,6 @@ namespace zg {
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 constexpr int kOwnWaves = 2048;     // waves over the rows' own tiles: two per SIMD
-constexpr int kManyTiles = 2;       // fewest tiles of a piece of the prefix for 128 queries
-constexpr int kPrefixGroups = 256;  // about so many over the prefix
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
 constexpr int kCus = 256;
 constexpr int kJoin = 8;             // pieces that a thread of the join has under way
@@ -925,13 +924,13 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_attn_many_kernel(Pag
 // Workgroup (kv head, row, four accumulators): a thread owns 16 bytes of the
 // pieces, (accumulator, quarter, query), and every n-th piece; the n threads
 // of one item are joined at the end, in order.
-template <bool IO, int D, int W>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, Cut c) {
-    __shared__ v4f parts[256];
-    __shared__ float2 stats[256];
+template <bool IO, int D, int W, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnArgs a, Cut c) {
+    __shared__ v4f parts[THREADS];
+    __shared__ float2 stats[THREADS];
     const uint32_t kvh = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
     const Run run = c.runs[r * a.pool.kv_heads + kvh];
-    const uint32_t items = 16 * a.group, n = 256 / items, item = tid % items, nth = tid / items;
+    const uint32_t items = 16 * a.group, n = THREADS / items, item = tid % items, nth = tid / items;
     const uint32_t col = item % a.group, fq = blockIdx.z * 16 + item / a.group;
     const uint32_t chunks = c.chunks, pieces = chunks + run.heads + run.mids + run.tails;
     if (a.lengths[r] < 0) return;
@@ -1021,10 +1020,22 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
     c.blocks = (int)(((uint64_t)rows * group + c.block - 1) / c.block);
     c.prefix_tiles = (int)((prefix_tokens + tile - 1) / tile);
     if (c.prefix_tiles) {
-        const int least = c.block == kManyQueries ? kManyTiles : 4;  // tiles of a piece
-        const int want = std::max(1, std::min((c.prefix_tiles + least - 1) / least,
-                                              kPrefixGroups / std::max(1, kv_heads * c.blocks)));
+        // More pieces run side by side, and each costs the join: with T tiles
+        // in all, a tile taking some 2 us and a piece of 128 queries adding
+        // 0.1 us (256-element heads), sqrt(20 T) pieces.  32 rows over 8192
+        // tokens: 256 pieces 25 + 12 us, 128 pieces 21 + 8; over 2048: 64
+        // pieces 15 + 6, 32 pieces 19 + 4.  A piece of few queries is cheap: one
+        // tile for each wave.
+        const int share = kv_heads * c.blocks;
+        const int most = c.block == kManyQueries ? (int)std::sqrt(20.0 * c.prefix_tiles * share) / share
+                                                 : std::min((c.prefix_tiles + 3) / 4, kCus / share);
+        const int want = std::max(1, std::min({most, c.prefix_tiles, kCus / share}));
         c.chunk_tiles = (c.prefix_tiles + want - 1) / want;
+        // many queries take tiles in pairs; one piece to a CU
+        if (c.block == kManyQueries && c.chunk_tiles % 2) {
+            const int less = std::max(2, c.chunk_tiles - 1);
+            c.chunk_tiles = (c.prefix_tiles + less - 1) / less * share <= kCus ? less : c.chunk_tiles + 1;
+        }
         c.chunks = (c.prefix_tiles + c.chunk_tiles - 1) / c.chunk_tiles;
     }
     // eight waves' queries may not fit the LDS (16 to a kv head, in three parts)
@@ -1093,7 +1104,13 @@ static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
     kernel<<<many ? std::max(over_prefix, kCus) : over_prefix + c.groups, 64 * waves, lds, st>>>(a, c);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    paged_join_kernel<IO, D, F::kWide><<<dim3(a.pool.kv_heads, a.rows, D / 64), 256, 0, st>>>(a, c);
+    // Few workgroups or many pieces: more threads, and fewer pieces for each.
+    // One row of 32768 tokens (8 workgroups) 15.8 -> 8.7 us, 8 rows over a
+    // prefix of 32768 (64) 10.4 -> 6.5, 32 rows over 131072 in 128 pieces
+    // (256) 12.3 -> 9.1; with 22 pieces there 4.2 -> 6.4.
+    const dim3 grid(a.pool.kv_heads, a.rows, D / 64);
+    if ((size_t)grid.x * grid.y * grid.z <= 64 || c.chunks > 64) paged_join_kernel<IO, D, F::kWide, 1024><<<grid, 1024, 0, st>>>(a, c);
+    else paged_join_kernel<IO, D, F::kWide, 256><<<grid, 256, 0, st>>>(a, c);
     return hipGetLastError();
 }
 
