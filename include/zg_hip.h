@@ -685,7 +685,8 @@ typedef struct zg_logit_rules {
  * history and counts history_lengths[r] up, while history_stride has room;
  * it needs a history and greedy.  No counterpart in the reference, whose
  * readout is greedy_finite alone (core/src/numerics.rs:124-140).  At most
- * 65535 rows and a vocabulary of 2^30; at most 65535 biases a row.  workspace
+ * 65535 rows, a vocabulary of 2^30, 65535 biases a row and a history_stride
+ * of 2^28.  workspace
  * of zg_logits_adjust_workspace_bytes bytes, 16-byte aligned, needed with
  * greedy (else NULL), one for each call that may run at the same time.
  * Asynchronous. */

@@ -1,14 +1,29 @@
 // Penalties, biases and masks on a batch's logits, and the highest one left
 // (include/zg_hip.h, zg_logits_adjust_device).
+//
+// A row's logits are read and written once.  Only the tokens in the history
+// and the biases change, so a workgroup gathers those of its slice of the
+// vocabulary in LDS and lists them, a thread forms the new value of each, in
+// 64 bits and rounded once, and the values are laid over the logits on their
+// way from registers to memory.  A history is read by every slice's
+// workgroup, which keeps a few tokens of each hundred: a wave first packs
+// those together (a ballot and a count of lower lanes, no atomics) and then
+// takes them a lane each.  The count of a token is a sum of integers and the
+// list's order of no account, so the order of the LDS atomics does not matter;
+// the biases of one token are summed in their order.
 #include "zg_paged.hpp"
 
 namespace zg {
 
-constexpr int kLogitSlice = 4096;  // tokens of a row per workgroup
-constexpr uint32_t kSeen = 0x80000000u;
+// A token's word: it is in the history; it has a bias; it has several; the
+// other bits count its generated occurrences (a history holds at most 2^28).
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kSeveral = 0x20000000u, kCount = kSeveral - 1;
+constexpr int kLeastSlice = 1024;
+constexpr int kBatch = 8;    // history loads of a thread under way
+constexpr int kList = 1024;  // listed tokens of a slice; where there are more, all are looked at
 
-// Order of two candidates of the greedy readout: the higher value, the lower
-// index of equal ones.  Index -1: none.
+// A candidate of the greedy readout: the higher value wins, of equal ones the
+// lower index.  Index -1: none.
 struct Best {
     float v;
     int i;
@@ -27,93 +42,204 @@ __device__ __forceinline__ Best wave_best(Best b) {
     return b;
 }
 
-// Workgroup (slice, row).  The row's history and biases that fall into the
-// slice are gathered in LDS: per token the count of its generated
-// occurrences (the top bit: it is in the history at all) and the index of
-// its first bias; then the slice's logits pass through registers once.
 template <bool BF16>
-__global__ __launch_bounds__(256) void logits_adjust_kernel(LogitArgs a, int slices) {
-    __shared__ uint32_t count[kLogitSlice];
-    __shared__ int bias[kLogitSlice];
-    __shared__ int twice;
-    __shared__ Best found[4];
+__device__ __forceinline__ float load_logit(const void* p, size_t at) {
+    if constexpr (BF16) return bf16_to_f32(((const uint16_t*)p)[at]);
+    else return ((const float*)p)[at];
+}
+
+// The lanes before this one that are in `lanes`.
+__device__ __forceinline__ int lanes_before(uint64_t lanes) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
+}
+
+// Workgroup (slice, row) of T threads and 4 V tokens a thread, four
+// neighbouring ones at a time.  WHOLE: four logits are loaded and stored at
+// once, which the rows' alignment must allow.
+template <bool BF16, bool WHOLE, int T, int V>
+__global__ __launch_bounds__(T) void logits_adjust_kernel(LogitArgs a, int slices) {
+    constexpr int SLICE = 4 * T * V, WAVES = T / 64;
+    static_assert(SLICE <= 32768, "offsets and a flag in 16 bits");
+    __shared__ __align__(16) uint32_t value[SLICE];   // a token's word, then its new value
+    __shared__ uint32_t touched[SLICE / 32];          // the listed tokens
+    __shared__ uint16_t list[kList];
+    __shared__ uint16_t hits[WAVES][64 * kBatch];     // a wave's history tokens in the slice, top bit: generated
+    __shared__ uint16_t bias_of[SLICE];               // one of a token's biases
+    __shared__ int listed;
+    __shared__ Best found[WAVES];
     const size_t r = blockIdx.y;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const zg_logit_rules& u = a.rules;
+    const size_t first = (size_t)blockIdx.x * SLICE;
+    const int n = (int)min((size_t)SLICE, a.vocab - first);
+    const size_t in = r * a.ld + first, out = r * a.out_ld + first;
+
+    // Everything that does not hang on something else is asked for at once: the
+    // row's numbers, the first of its history and biases (as much of them as
+    // their strides hold, whatever their lengths say) and the logits.
     const int held = u.history ? u.history_lengths[r] : 0;
+    const int prompt = u.prompt_lengths ? u.prompt_lengths[r] : 0;
+    const int given = u.bias_ids ? u.bias_lengths[r] : 0;
+    const float rep = u.repetition ? u.repetition[r] : 1.0f;
+    const float freq = u.frequency ? u.frequency[r] : 0.0f, pres = u.presence ? u.presence[r] : 0.0f;
+    const int mask_row = u.masks ? u.mask_of ? u.mask_of[r] : (int)r : -1;
+    const int32_t* const history = u.history + (u.history ? r * u.history_stride : 0);
+    const int room = u.history ? (int)u.history_stride : 0;
+    uint32_t id[kBatch];
+    auto load_history = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = from + k * T + tid;
+            id[k] = i < room ? (uint32_t)history[i] : 0xffffffffu;
+        }
+    };
+    load_history(0);
+    const int32_t* const ids = u.bias_ids + (u.bias_ids ? r * u.bias_stride : 0);
+    const float* const add = u.bias_values + (u.bias_ids ? r * u.bias_stride : 0);
+    const uint32_t bias_id = u.bias_ids && tid < (int)u.bias_stride ? (uint32_t)ids[tid] : 0xffffffffu;
+    v4f x[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int i = 4 * (k * T + tid);
+        x[k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (i < n) {
+            if (WHOLE && i + 4 <= n) x[k] = load4<BF16>(a.logits, in + i);
+            else
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < n) x[k][j] = load_logit<BF16>(a.logits, in + i + j);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) *(v4u*)&value[4 * (k * T + tid)] = v4u{0, 0, 0, 0};
+    if (tid < SLICE / 32) touched[tid] = 0;
+    if (tid == 0) listed = 0;
+    const bool none = mask_row >= 0 && (size_t)mask_row >= u.mask_rows;  // a mask that is not there allows nothing
+    const uint32_t* mask = mask_row >= 0 && !none ? u.masks + (size_t)mask_row * u.mask_stride + first / 32 : nullptr;
+    uint32_t allowed[V];  // of the four tokens, and of those past the vocabulary none
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int i = 4 * (k * T + tid);
+        allowed[k] = none || i >= n ? 0u : mask ? mask[i >> 5] >> (i & 31) : 0xfu;
+        if (i + 4 > n && i < n) allowed[k] &= (1u << (n - i)) - 1;
+    }
     if (held < 0) return;
-    const size_t first = (size_t)blockIdx.x * kLogitSlice;
-    const int n = (int)min((size_t)kLogitSlice, a.vocab - first);
-    for (int i = tid; i < kLogitSlice; i += 256) {
-        count[i] = 0;
-        bias[i] = 0x7fffffff;
-    }
-    if (tid == 0) twice = 0;
-    __syncthreads();
-    if (u.history) {
-        const int32_t* tokens = u.history + r * u.history_stride;
-        const size_t len = min((size_t)held, u.history_stride);
-        const int prompt = u.prompt_lengths ? u.prompt_lengths[r] : 0;
-        for (size_t i = tid; i < len; i += 256) {
-            const uint32_t at = (uint32_t)tokens[i] - (uint32_t)first;
-            if ((uint32_t)tokens[i] < a.vocab && at < (uint32_t)n) {
-                atomicOr(&count[at], kSeen);
-                if ((long long)i >= prompt) atomicAdd(&count[at], 1u);
+    const int biases = u.bias_ids ? max(0, min(given, (int)u.bias_stride)) : 0, tokens = min(held, room);
+    const bool changes = tokens > 0 || biases > 0;
+    if (changes) {
+        __syncthreads();
+        auto enlist = [&](uint32_t at) {
+            const uint32_t bit = 1u << (at & 31);
+            if (atomicOr(&touched[at >> 5], bit) & bit) return;
+            const int k = atomicAdd(&listed, 1);
+            if (k < kList) list[k] = (uint16_t)at;
+        };
+        for (int from = 0; from < tokens; from += kBatch * T) {
+            int got = 0;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = from + k * T + tid;
+                const uint32_t at = id[k] - (uint32_t)first;  // below n: it is in the vocabulary
+                const bool hit = at < (uint32_t)n && i < tokens;
+                const uint64_t lanes = __ballot(hit);
+                if (hit) hits[wave][got + lanes_before(lanes)] = (uint16_t)(at | (i >= prompt ? 0x8000u : 0u));
+                got += __popcll(lanes);
             }
+            if (from + kBatch * T < tokens) load_history(from + kBatch * T);
+            __builtin_amdgcn_wave_barrier();
+            for (int k = lane; k < got; k += 64) {
+                const uint32_t at = hits[wave][k] & 0x7fffu, made = hits[wave][k] >> 15;
+                enlist(at);
+                // the top bit is set by or, not by sum: it is there once
+                atomicOr(&value[at], kSeen);
+                if (made) atomicAdd(&value[at], 1u);
+            }
+            __builtin_amdgcn_wave_barrier();
         }
+        // any of a token's biases stays in bias_of; the others then find it
+        // there and mark the token
+        auto each_bias = [&](auto then) {
+            for (int i = tid; i < biases; i += T) {
+                const uint32_t at = (i < T ? bias_id : (uint32_t)ids[i]) - (uint32_t)first;
+                if (at < (uint32_t)n) then(i, at);
+            }
+        };
+        each_bias([&](int i, uint32_t at) {
+            enlist(at);
+            atomicOr(&value[at], kBiased);
+            bias_of[at] = (uint16_t)i;
+        });
+        __syncthreads();
+        if (biases) {
+            each_bias([&](int i, uint32_t at) {
+                if (bias_of[at] != i) atomicOr(&value[at], kSeveral);
+            });
+            __syncthreads();
+        }
+#pragma unroll 1
+        for (int k = tid; k < (listed <= kList ? listed : n); k += T) {
+            const int i = listed <= kList ? list[k] : k;
+            if (!(touched[i >> 5] >> (i & 31) & 1u)) continue;
+            const uint32_t c = value[i];
+            double v = (double)load_logit<BF16>(a.logits, in + i);
+            if (c & kSeen) v = v > 0.0 ? v / (double)rep : v * (double)rep;
+            if (c & kCount) v = v - (double)freq * (double)(c & kCount) - (double)pres;
+            if (c & kSeveral) {
+                double sum = 0.0;
+                for (int j = 0; j < biases; ++j)
+                    if (ids[j] == (int)(first + i)) sum += (double)add[j];
+                v += sum;
+            } else if (c & kBiased) {
+                v += (double)add[bias_of[i]];
+            }
+            float y = (float)v;
+            if constexpr (BF16) y = bf16_to_f32(to_bf16(y));
+            value[i] = __float_as_uint(y);
+        }
+        __syncthreads();
     }
-    const int32_t* ids = u.bias_ids ? u.bias_ids + r * u.bias_stride : nullptr;
-    const float* values = u.bias_ids ? u.bias_values + r * u.bias_stride : nullptr;
-    const int nb = ids ? max(0, min(u.bias_lengths[r], (int)u.bias_stride)) : 0;
-    for (int i = tid; i < nb; i += 256) {
-        const uint32_t at = (uint32_t)ids[i] - (uint32_t)first;
-        if ((uint32_t)ids[i] < a.vocab && at < (uint32_t)n && atomicMin(&bias[at], i) != 0x7fffffff) twice = 1;
-    }
-    __syncthreads();
-    const double rep = u.repetition ? (double)u.repetition[r] : 1.0;
-    const double freq = u.frequency ? (double)u.frequency[r] : 0.0, pres = u.presence ? (double)u.presence[r] : 0.0;
-    int mask_row = -1;
-    if (u.masks) mask_row = u.mask_of ? u.mask_of[r] : (int)r;
-    // a mask that is not there allows nothing
-    const bool none = mask_row >= 0 && (size_t)mask_row >= u.mask_rows;
-    const uint32_t* mask = mask_row >= 0 && !none ? u.masks + (size_t)mask_row * u.mask_stride : nullptr;
-    Best best{0.0f, -1};
+
+    Best best{-INFINITY, -1};  // indices ascend: a later one takes a higher value
     bool odd = false;
-    for (int i = tid; i < n; i += 256) {
-        const size_t t = first + i;
-        float x;
-        if constexpr (BF16) x = bf16_to_f32(((const uint16_t*)a.logits)[r * a.ld + t]);
-        else x = ((const float*)a.logits)[r * a.ld + t];
-        const uint32_t c = count[i];
-        const int b = bias[i];
-        if (c || b != 0x7fffffff) {
-            double v = (double)x;
-            if (c) v = v > 0.0 ? v / rep : v * rep;
-            if (c & ~kSeen) v = v - freq * (double)(c & ~kSeen) - pres;
-            if (b != 0x7fffffff) {
-                double add = (double)values[b];
-                if (twice)
-                    for (int j = b + 1; j < nb; ++j)
-                        if (ids[j] == (int)t) add += (double)values[j];
-                v += add;
-            }
-            x = (float)v;
-            if constexpr (BF16) x = bf16_to_f32(to_bf16(x));
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int i = 4 * (k * T + tid);
+        if (changes) {
+            const uint32_t t = touched[i >> 5] >> (i & 31);
+            const v4u w = *(const v4u*)&value[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (t >> j & 1u) x[k][j] = __uint_as_float(w[j]);
         }
-        const bool allowed = !none && (!mask || (mask[t >> 5] >> (t & 31) & 1u));
-        if (!allowed) x = -INFINITY;
-        if constexpr (BF16) ((uint16_t*)a.out)[r * a.out_ld + t] = to_bf16(x);
-        else ((float*)a.out)[r * a.out_ld + t] = x;
-        odd |= x != x || x == INFINITY;
-        if (x > -INFINITY) best = better(best, Best{x, (int)t});
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!(allowed[k] >> j & 1u)) x[k][j] = -INFINITY;
+            odd |= !(x[k][j] < INFINITY);
+            if (x[k][j] > best.v) best = Best{x[k][j], (int)first + i + j};
+        }
+        if (i >= n) continue;
+        if (WHOLE && i + 4 <= n) {
+            if constexpr (BF16)  // the values are bfloat16 already
+                *(uint2*)((uint16_t*)a.out + out + i) =
+                    make_uint2(__builtin_amdgcn_perm(__float_as_uint(x[k][1]), __float_as_uint(x[k][0]), 0x07060302u),
+                               __builtin_amdgcn_perm(__float_as_uint(x[k][3]), __float_as_uint(x[k][2]), 0x07060302u));
+            else
+                store4<false>(a.out, out + i, x[k]);
+        } else {
+            for (int j = 0; j < 4; ++j) {
+                if (i + j >= n) break;
+                if constexpr (BF16) ((uint16_t*)a.out)[out + i + j] = (uint16_t)(__float_as_uint(x[k][j]) >> 16);
+                else ((float*)a.out)[out + i + j] = x[k][j];
+            }
+        }
     }
-    if (a.status && __any(odd) && (tid & 63) == 0) atomicOr(a.status, ZG_STATUS_NONFINITE);
+    if (a.status && __any(odd) && lane == 0) atomicOr(a.status, ZG_STATUS_NONFINITE);
     if (!a.greedy) return;
     best = wave_best(best);
-    if ((tid & 63) == 0) found[tid >> 6] = best;
+    if (lane == 0) found[wave] = best;
     __syncthreads();
     if (tid == 0) {
-        best = better(better(found[0], found[1]), better(found[2], found[3]));
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) best = better(best, found[w]);
         ((Best*)a.workspace)[r * slices + blockIdx.x] = best;
     }
 }
@@ -135,15 +261,30 @@ __global__ __launch_bounds__(64) void logits_greedy_kernel(LogitArgs a, int slic
     }
 }
 
-static int slices_of(size_t vocab) { return (int)((vocab + kLogitSlice - 1) / kLogitSlice); }
+static int slices_of(size_t vocab, int slice) { return (int)((vocab + slice - 1) / slice); }
 
-size_t logits_workspace(size_t rows, size_t vocab) { return rows * slices_of(vocab) * sizeof(Best); }
+size_t logits_workspace(size_t rows, size_t vocab) { return rows * slices_of(vocab, kLeastSlice) * sizeof(Best); }
+
+template <bool BF16, bool WHOLE>
+static int adjust(const LogitArgs& a, hipStream_t st) {
+    // Every slice reads the row's history, so few long slices cost less, while
+    // one row alone wants many short ones: with a vocabulary of 151936 slices
+    // of 1024 and of 4096 tokens take 5.9 and 6.8 us at 1 row (600 tokens of
+    // history), 8.6 and 7.2 at 3 (4000), 9.0 and 8.0 at 8 (2000), 21.5 and 17.0
+    // at 32 (2500); slices of 8192, two workgroups to a CU, 19.6 at 32.
+    const int slice = a.rows * slices_of(a.vocab, 4096) >= 96 ? 4096 : kLeastSlice, slices = slices_of(a.vocab, slice);
+    const dim3 grid(slices, (unsigned)a.rows);
+    if (slice == 4096) logits_adjust_kernel<BF16, WHOLE, 512, 2><<<grid, 512, 0, st>>>(a, slices);
+    else logits_adjust_kernel<BF16, WHOLE, 256, 1><<<grid, 256, 0, st>>>(a, slices);
+    return slices;
+}
 
 hipError_t logits_adjust(const LogitArgs& a, hipStream_t st) {
-    const int slices = slices_of(a.vocab);
-    const dim3 grid(slices, (unsigned)a.rows);
-    if (a.bf16) logits_adjust_kernel<true><<<grid, 256, 0, st>>>(a, slices);
-    else logits_adjust_kernel<false><<<grid, 256, 0, st>>>(a, slices);
+    // four logits at once where every row starts at a multiple of four
+    const size_t four = a.bf16 ? 8 : 16;
+    const bool whole = ((uintptr_t)a.logits | (uintptr_t)a.out) % four == 0 && a.ld % 4 == 0 && a.out_ld % 4 == 0;
+    const int slices = a.bf16 ? (whole ? adjust<true, true>(a, st) : adjust<true, false>(a, st))
+                              : (whole ? adjust<false, true>(a, st) : adjust<false, false>(a, st));
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.greedy) return e;
     logits_greedy_kernel<<<(unsigned)a.rows, 64, 0, st>>>(a, slices);

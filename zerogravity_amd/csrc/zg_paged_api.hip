@@ -16,6 +16,7 @@ namespace {
 
 constexpr size_t kMaxRows = 4096;
 constexpr size_t kMaxRowTokens = (size_t)1 << 30;
+constexpr size_t kMaxHistory = (size_t)1 << 28;  // what zg_logits.hip's words count
 constexpr size_t kMaxStride = (size_t)1 << 32;  // elements: offsets of 2^31 rows stay within 64 bits
 
 // The context's device for the length of a call; the caller's comes back.
@@ -277,9 +278,9 @@ int zg_logits_adjust_device(zg_ctx* ctx, size_t rows, size_t vocab, const void* 
         if (std::max({ld, out_ld, u.mask_stride, u.mask_rows}) > kMaxStride)
             return fail(ctx, ZG_E_LIMIT, "logits and masks with strides of at most 2^32");
         if ((u.history == nullptr) != (u.history_lengths == nullptr) ||
-            (u.history && (u.history_stride == 0 || u.history_stride > kMaxRowTokens)) ||
+            (u.history && (u.history_stride == 0 || u.history_stride > kMaxHistory)) ||
             (!u.history && (u.prompt_lengths || u.repetition || u.frequency || u.presence)))
-            return fail(ctx, ZG_E_MALFORMED, "penalties need a history of 1 to 2^30 tokens a row and its lengths");
+            return fail(ctx, ZG_E_MALFORMED, "penalties need a history of 1 to 2^28 tokens a row and its lengths");
         if ((u.bias_ids == nullptr) != (u.bias_values == nullptr) || (u.bias_ids == nullptr) != (u.bias_lengths == nullptr) ||
             (u.bias_ids && u.bias_stride == 0))
             return fail(ctx, ZG_E_MALFORMED, "biases need ids, values and lengths");
