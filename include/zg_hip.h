@@ -599,7 +599,7 @@ int zg_paged_admit(const zg_paged_kv* cache, const zg_paged_rows* rows, const in
  * [tokens][q_heads * head_dim] of dtype, contiguous; it may be q itself where
  * q is contiguous.  positions [tokens] (device) counts from the prefix's
  * first token, so a row's first own token is at rows->prefix_tokens;
- * negative: the token is skipped, nothing of it is read or written.
+ * negative: the token is skipped, nothing is written for it.
  * token_rows [tokens] (device) is each token's row, NULL: token t belongs to
  * row t.  rotate 0 to head_dim, a multiple of 8.  The positions of one row in
  * one call differ from each other; which of two tokens at one place stays is

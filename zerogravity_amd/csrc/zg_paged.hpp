@@ -127,4 +127,16 @@ __device__ __forceinline__ void store4(void* base, size_t at, v4f x) {
     }
 }
 
+// The value of the lane 16 or 32 further on (xor), without the LDS.
+template <int XOR>
+__device__ __forceinline__ float other_quarter(float x) {
+    if constexpr (XOR == 16) {
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+        return __int_as_float((threadIdx.x & 16) ? y[0] : y[1]);
+    } else {
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+        return __int_as_float((threadIdx.x & 32) ? y[0] : y[1]);
+    }
+}
+
 }  // namespace zg

@@ -159,18 +159,6 @@ struct Weights {
     }
 };
 
-// The value of the lane 16 or 32 further on (xor), without the LDS.
-template <int XOR>
-__device__ __forceinline__ float other_quarter(float x) {
-    if constexpr (XOR == 16) {
-        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
-        return __int_as_float((threadIdx.x & 16) ? y[0] : y[1]);
-    } else {
-        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
-        return __int_as_float((threadIdx.x & 32) ? y[0] : y[1]);
-    }
-}
-
 // A tile's weights e^(s - m) from its scores, m the query's reference: the
 // sums are brought to a new one only when a score passes the old one by
 // 2^kRaise, which 32-bit sums hold with ease.
@@ -259,11 +247,12 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const Wei
     }
 }
 
-// Tiles tile, tile + step, ... before `end` of one table added to the sums.
+// Tiles tile, tile + step, ... before `end` of one table added to the sums;
+// page is what the table says of the first.
 template <bool IO, bool KV, int D, int MT>
 __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* queries, int n, const int32_t* table,
-                                          uint32_t tokens, int tile, int end, int step, int kvh, Sums<D, MT>& s,
-                                          int& bad) {
+                                          uint32_t tokens, int tile, int end, int step, int kvh, uint32_t page,
+                                          Sums<D, MT>& s, int& bad) {
     using F = Form<IO, KV, D>;
     constexpr int W = F::kWide, H = F::kHalves, N = F::kMine;
     constexpr int ES = KV ? 2 : 4, VR = W * ES / 4;  // registers of a value row per load
@@ -272,8 +261,6 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
     const char* const keys = (const char*)a.pool.keys;
     const char* const values = (const char*)a.pool.values;
     constexpr uint32_t kAll = H == 2 ? 0xffffffffu : 0xffffu;
-    if (tile >= end) return;
-    uint32_t page = peek<F::kTile>(a.pool, table, tokens, tile, lane);
     for (; tile < end; tile += step) {
         const Place at = resolve<F::kTile>(a.pool, page, tokens, tile, lane);
         if (at.stray) bad |= ZG_STATUS_PAGE;
@@ -525,14 +512,15 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
             return r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
         }
     } who{a.q, a, block * 16 * MT, queries - 1, kvh};
+    const int first = chunk * c.chunk_tiles;
+    const uint32_t page = peek<Form<IO, KV, D>::kTile>(a.pool, a.prefix, a.prefix_tokens, first + wave, lane);
     stage_queries<IO, KV, D>((v4u*)lds, 16 * MT, tid, 256, a.scale * kLog2e, who);
     __syncthreads();
     Sums<D, MT> s;
     s.clear();
     int bad = 0;
-    const int first = chunk * c.chunk_tiles;
     add_tiles<IO, KV, D, MT>(a, (const v4u*)lds, 16 * MT, a.prefix, a.prefix_tokens, first + wave,
-                             min(first + c.chunk_tiles, c.prefix_tiles), 4, kvh, s, bad);
+                             min(first + c.chunk_tiles, c.prefix_tiles), 4, kvh, page, s, bad);
     if (bad && a.status) atomicOr(a.status, bad);
     __syncthreads();
     gather_waves<D, MT>(s, 4, wave, lane, lds);
@@ -647,10 +635,11 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
             size_t first;
             __device__ size_t operator()(int m) const { return first + (size_t)m * D; }
         } who{a.q, r * a.q_stride + (size_t)kvh * a.group * D};
+        const int32_t* const table = a.table + (size_t)r * a.stride;
+        const uint32_t here = own_tokens(a, r), page = peek<F::kTile>(a.pool, table, here, (int)tile, lane);
         stage_queries<IO, KV, D>(queries, a.group, lane, 64, a.scale * kLog2e, who);
         same_wave();
-        add_tiles<IO, KV, D, 1>(a, queries, a.group, a.table + (size_t)r * a.stride, own_tokens(a, r), (int)tile,
-                                (int)upto_tile, 1, (int)kvh, s, bad);
+        add_tiles<IO, KV, D, 1>(a, queries, a.group, table, here, (int)tile, (int)upto_tile, 1, (int)kvh, page, s, bad);
         __builtin_amdgcn_wave_barrier();
         t += upto_tile - tile;
         if (gathered) break;
