@@ -32,7 +32,6 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 constexpr int kOwnWaves = 2048;     // waves over the rows' own tiles: two per SIMD
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
 constexpr int kCus = 256;
-constexpr int kJoin = 8;             // pieces that a thread of the join has under way
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRaise = 8.0f;      // log2: how far a score may pass the reference before sums are rescaled
 
@@ -915,6 +914,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_attn_many_kernel(Pag
 // of one item are joined at the end, in order.
 template <bool IO, int D, int W, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnArgs a, Cut c) {
+    constexpr int kJoin = THREADS == 1024 ? 4 : 8;  // pieces that a thread has under way
     __shared__ v4f parts[THREADS];
     __shared__ float2 stats[THREADS];
     const uint32_t kvh = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
@@ -964,11 +964,13 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnArgs a, Cu
     __syncthreads();
     if (tid < items) {
         float to = top;
+#pragma unroll 4
         for (uint32_t i = 1; i < n; ++i) to = fmaxf(to, stats[tid + i * items].x);
         const float sub = to == -INFINITY ? 0.0f : to;
         const float keep = __builtin_amdgcn_exp2f(top == to ? 0.0f : top - sub);
         l *= keep;
         o *= keep;
+#pragma unroll 4
         for (uint32_t i = 1; i < n; ++i) {
             const float2 y = stats[tid + i * items];
             const float e = __builtin_amdgcn_exp2f(y.x == to ? 0.0f : y.x - sub);
@@ -1094,9 +1096,9 @@ static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // Few workgroups or many pieces: more threads, and fewer pieces for each.
-    // One row of 32768 tokens (8 workgroups) 15.8 -> 8.7 us, 8 rows over a
-    // prefix of 32768 (64) 10.4 -> 6.5, 32 rows over 131072 in 128 pieces
-    // (256) 12.3 -> 9.1; with 22 pieces there 4.2 -> 6.4.
+    // One row of 32768 tokens (8 workgroups) 15.9 -> 8.9 us, of 2048 5.8 -> 4.8,
+    // 8 rows over a prefix of 32768 (64) 10.6 -> 6.1, 32 rows over 131072 in
+    // 128 pieces (256) 13.0 -> 8.9; with 22 pieces there 4.2 -> 6.4.
     const dim3 grid(a.pool.kv_heads, a.rows, D / 64);
     if ((size_t)grid.x * grid.y * grid.z <= 64 || c.chunks > 64) paged_join_kernel<IO, D, F::kWide, 1024><<<grid, 1024, 0, st>>>(a, c);
     else paged_join_kernel<IO, D, F::kWide, 256><<<grid, 256, 0, st>>>(a, c);
