@@ -601,7 +601,7 @@ int zg_paged_admit(const zg_paged_kv* cache, const zg_paged_rows* rows, const in
  * first token, so a row's first own token is at rows->prefix_tokens;
  * negative: the token is skipped, nothing is written for it.
  * token_rows [tokens] (device) is each token's row, NULL: token t belongs to
- * row t.  rotate 0 to head_dim, a multiple of 8.  The positions of one row in
+ * row t.  tokens 1 to 2^24 - 1; rotate 0 to head_dim, a multiple of 8.  The positions of one row in
  * one call differ from each other; which of two tokens at one place stays is
  * not defined.  A row or position outside the table (ZG_STATUS_POSITION) or a
  * page outside the pool (ZG_STATUS_PAGE) stores no key and value; the query is
@@ -631,7 +631,10 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
  * zeros; a negative length leaves the row's out as it was.  A length past the
  * row's table is cut to it (ZG_STATUS_POSITION); tokens of a page outside the
  * pool are left out (ZG_STATUS_PAGE).  What slots past a row's length hold
- * does not matter.  workspace of zg_paged_attn_workspace_bytes bytes (0 for
+ * does not matter.  NaN and infinities among the tokens come through as the
+ * formula has them, but that an infinite key or value of a ZG_BF16 cache
+ * may make what it enters NaN (the parts of a 32-bit factor can be 0).
+ * |scale| below 2^127.  workspace of zg_paged_attn_workspace_bytes bytes (0 for
  * arguments that the call refuses), 16-byte aligned, is written and read by
  * the call: calls, and replays of captured ones, that may run at the same
  * time need one each.  A captured call keeps prefix_tokens and the pointers,
@@ -646,7 +649,7 @@ int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_r
  * prompt first, history_lengths[r] of them (a negative length: the row is
  * left out of the call, its logits and id as they were), the first
  * prompt_lengths[r] (NULL: none) the prompt.  Ids outside the vocabulary
- * count for nothing.  Per row: repetition r > 0 divides a positive and
+ * count for nothing, nor do the entries past a length, which may be read.  Per row: repetition r > 0 divides a positive and
  * multiplies any other logit of a token in the history; frequency f and
  * presence p take f * count + p from a token generated `count` > 0 times
  * (after the prompt).  bias_ids, bias_values [rows][bias_stride],

@@ -124,3 +124,26 @@ def test_python_forms_refuse_what_is_not_the_pools():
         sampling.rules(repetition=torch.zeros(2, dtype=torch.float64))
     with pytest.raises(L.ZgError):
         sampling.rules(bias_ids=torch.zeros(2, 3, dtype=torch.int32), bias_values=torch.zeros(2, 4))
+
+
+def test_table_views_end_inside_their_storage():
+    """A row of the table counts as long as the row stride, the last row too."""
+    wide = torch.zeros(5, 9, dtype=torch.int32)
+    assert paged.rows(wide[:, :4]).stride == paged.rows(wide).stride == 9
+    assert paged.rows(wide[3:4, 5:]).stride == 4  # one row is as long as the view
+    paged.rows(wide[:4, 5:])
+    with pytest.raises(L.ZgError):
+        paged.rows(wide[:, 5:])
+    with pytest.raises(L.ZgError):
+        paged.rows(wide[1:, 1:])
+
+
+def test_streams_of_another_device_are_refused():
+    from types import SimpleNamespace
+
+    from zerogravity_amd import _torch
+    ctx = SimpleNamespace(device=0)
+    here = SimpleNamespace(device=torch.device("cuda", 0))
+    assert _torch.stream_of(ctx, here) is here
+    with pytest.raises(L.ZgError):
+        _torch.stream_of(ctx, SimpleNamespace(device=torch.device("cuda", 1)))

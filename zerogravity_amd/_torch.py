@@ -41,7 +41,11 @@ def on_device(ctx, t, what):
 def stream_of(ctx, stream):
     """The torch stream of one call: the one given, else the current one."""
     import torch
-    return torch.cuda.current_stream(ctx.device) if stream is None else stream
+    if stream is None:
+        return torch.cuda.current_stream(ctx.device)
+    if stream.device.index != ctx.device:
+        malformed("stream: of the context's device")
+    return stream
 
 
 def room(ctx, stream, workspace, need):

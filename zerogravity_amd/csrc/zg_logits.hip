@@ -145,7 +145,7 @@ __global__ __launch_bounds__(T) void logits_adjust_kernel(LogitArgs a, int slice
                 got += __popcll(lanes);
             }
             if (from + kBatch * T < tokens) load_history(from + kBatch * T);
-            __builtin_amdgcn_wave_barrier();
+            same_wave();
             for (int k = lane; k < got; k += 64) {
                 const uint32_t at = hits[wave][k] & 0x7fffu, made = hits[wave][k] >> 15;
                 enlist(at);
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(T) void logits_adjust_kernel(LogitArgs a, int slice
                 atomicOr(&value[at], kSeen);
                 if (made) atomicAdd(&value[at], 1u);
             }
-            __builtin_amdgcn_wave_barrier();
+            same_wave();
         }
         // any of a token's biases stays in bias_of; the others then find it
         // there and mark the token

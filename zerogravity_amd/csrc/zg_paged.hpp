@@ -127,6 +127,13 @@ __device__ __forceinline__ void store4(void* base, size_t at, v4f x) {
     }
 }
 
+// What a wave wrote to LDS, its other lanes read after this.
+__device__ __forceinline__ void same_wave() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The value of the lane 16 or 32 further on (xor), without the LDS.
 template <int XOR>
 __device__ __forceinline__ float other_quarter(float x) {

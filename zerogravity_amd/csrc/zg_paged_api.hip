@@ -16,6 +16,7 @@ namespace {
 
 constexpr size_t kMaxRows = 4096;
 constexpr size_t kMaxRowTokens = (size_t)1 << 30;
+constexpr size_t kMaxTokens = ((size_t)1 << 24) - 1;  // of 256 threads each in one launch
 constexpr size_t kMaxHistory = (size_t)1 << 28;  // what zg_logits.hip's words count
 constexpr size_t kMaxStride = (size_t)1 << 32;  // elements: offsets of 2^31 rows stay within 64 bits
 
@@ -167,8 +168,8 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
         if (!k || !v || !positions || tokens == 0 || k_stride < width || v_stride < width || k_stride % 4 ||
             v_stride % 4 || !aligned(k, four) || !aligned(v, four))
             return fail(ctx, ZG_E_MALFORMED, "paged append: keys, values and positions");
-        if (q_heads > 65536 || tokens > 0x7fffffffu || std::max({q_stride, q_head_stride, k_stride, v_stride}) > kMaxStride)
-            return fail(ctx, ZG_E_LIMIT, "paged append of at most 2^31 - 1 tokens and strides of 2^32");
+        if (q_heads > 65536 || tokens > kMaxTokens || std::max({q_stride, q_head_stride, k_stride, v_stride}) > kMaxStride)
+            return fail(ctx, ZG_E_LIMIT, "paged append of at most 2^24 - 1 tokens, 65536 query heads and strides of 2^32");
         if ((q_heads == 0) != (q == nullptr) || (q_heads == 0) != (q_out == nullptr) || q_head_stride % 4 ||
             q_stride % 4 || !aligned(q, four) || !aligned(q_out, four) ||
             (q_heads && (q_head_stride < cache->head_dim || q_stride < (q_heads - 1) * q_head_stride + cache->head_dim)))
@@ -231,7 +232,8 @@ int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_r
             return fail(ctx, ZG_E_MALFORMED, "paged attention: queries, lengths, workspace and outputs");
         if (std::max(q_stride, out_stride) > kMaxStride)
             return fail(ctx, ZG_E_LIMIT, "paged attention with strides of at most 2^32");
-        if (!std::isfinite(scale)) return fail(ctx, ZG_E_MALFORMED, "paged attention: the scale is finite");
+        if (!std::isfinite(2.0f * scale))  // the kernels count in log2
+            return fail(ctx, ZG_E_MALFORMED, "paged attention: twice the scale is finite");
         if (q == out && q_stride != out_stride)
             return fail(ctx, ZG_E_MALFORMED, "paged attention: outputs in place keep the queries' stride");
         zg::PagedAttnArgs a;

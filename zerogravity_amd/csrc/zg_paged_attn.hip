@@ -529,13 +529,6 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
         store_prefix<D>(a, c, kvh * c.chunks + chunk, block * 16 * MT + 16 * m + col, s.o[m], s.ref[m], s.l[m], quarter);
 }
 
-// What a wave wrote to LDS, its other lanes read after this.
-__device__ __forceinline__ void same_wave() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // LDS of own_block's table: 68 words for each wave, or one for all of them.
 __host__ __device__ inline size_t table_bytes(uint32_t rows, int waves) {
     return rows <= 64 ? (size_t)waves * 68 * 4 : ((size_t)(rows + 1 + waves) * 4 + 15) / 16 * 16;
@@ -639,7 +632,7 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
         stage_queries<IO, KV, D>(queries, a.group, lane, 64, a.scale * kLog2e, who);
         same_wave();
         add_tiles<IO, KV, D, 1>(a, queries, a.group, table, here, (int)tile, (int)upto_tile, 1, (int)kvh, page, s, bad);
-        __builtin_amdgcn_wave_barrier();
+        same_wave();
         t += upto_tile - tile;
         if (gathered) break;
         s.l[0] += __shfl_xor(s.l[0], 16, kWave);

@@ -29,14 +29,19 @@ def cache(keys, values):
 
 
 def rows(table, prefix=None, prefix_tokens=0):
-    """The zg_paged_rows of a table [rows, stride] (int32, row stride any) and
-    of the shared prefix's pages."""
+    """The zg_paged_rows of a table [rows, stride] (int32; a view's rows may lie
+    further apart, and then count as that long) and of the shared prefix's
+    pages."""
     if table.dim() != 2 or str(table.dtype) != "torch.int32" or (table.shape[1] > 1 and table.stride(1) != 1):
         malformed("page table: int32 [rows, pages]")
     if prefix is not None and (prefix.dim() != 1 or prefix.dtype != table.dtype or not prefix.is_contiguous() or
                                prefix.device != table.device):
         malformed("prefix pages: int32 [pages]")
     stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    # a length may ask for entries up to the row stride: the last row's are
+    # there too
+    if table.storage_offset() + table.shape[0] * stride > table.untyped_storage().nbytes() // 4:
+        malformed("page table: the last row's stride ends past the tensor's storage")
     r = L.PagedRows(table.data_ptr(), table.shape[0], stride,
                     prefix.data_ptr() if prefix is not None and prefix.numel() else None, prefix_tokens)
     r.tensors = (table, prefix)
