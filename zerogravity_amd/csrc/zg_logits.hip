@@ -48,9 +48,9 @@ __device__ __forceinline__ float load_logit(const void* p, size_t at) {
     else return ((const float*)p)[at];
 }
 
-// The lanes before this one that are in `lanes`.
-__device__ __forceinline__ int lanes_before(uint64_t lanes) {
-    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
+// `more` and the lanes before this one that are in `lanes`.
+__device__ __forceinline__ int lanes_before(uint64_t lanes, int more) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, (uint32_t)more));
 }
 
 // Workgroup (slice, row) of T threads and 4 V tokens a thread, four
@@ -125,6 +125,7 @@ __global__ __launch_bounds__(T) void logits_adjust_kernel(LogitArgs a, int slice
     if (held < 0) return;
     const int biases = u.bias_ids ? max(0, min(given, (int)u.bias_stride)) : 0, tokens = min(held, room);
     const bool changes = tokens > 0 || biases > 0;
+    const int made_from = max(0, min(prompt, tokens)) - 64 * wave;  // less the wave's part of a token's place
     if (changes) {
         __syncthreads();
         auto enlist = [&](uint32_t at) {
@@ -134,14 +135,17 @@ __global__ __launch_bounds__(T) void logits_adjust_kernel(LogitArgs a, int slice
             if (k < kList) list[k] = (uint16_t)at;
         };
         for (int from = 0; from < tokens; from += kBatch * T) {
+            if (from + kBatch * T > tokens)  // the last ones: what is past the end is no token
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+                    if (from + k * T + tid >= tokens) id[k] = 0xffffffffu;
             int got = 0;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                const int i = from + k * T + tid;
                 const uint32_t at = id[k] - (uint32_t)first;  // below n: it is in the vocabulary
-                const bool hit = at < (uint32_t)n && i < tokens;
+                const bool hit = at < (uint32_t)n;
                 const uint64_t lanes = __ballot(hit);
-                if (hit) hits[wave][got + lanes_before(lanes)] = (uint16_t)(at | (i >= prompt ? 0x8000u : 0u));
+                if (hit) hits[wave][lanes_before(lanes, got)] = (uint16_t)(at | (lane >= made_from - from - k * T ? 0x8000u : 0u));
                 got += __popcll(lanes);
             }
             if (from + kBatch * T < tokens) load_history(from + kBatch * T);
