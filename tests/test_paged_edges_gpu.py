@@ -74,6 +74,42 @@ def test_captured_calls_over_a_prefix(ctx, io, cache):
         assert torch.equal(out, eager), step
 
 
+@pytest.mark.parametrize("io,cache", TYPES)
+@pytest.mark.parametrize("rows,kv_heads,group,dim,prefix", [(65, 2, 16, 256, 1601), (65, 4, 5, 128, 2401),
+                                                           (100, 8, 1, 64, 3601), (40, 1, 16, 256, 4999)])
+def test_many_queries_over_a_prefix(ctx, io, cache, rows, kv_heads, group, dim, prefix):
+    """So many that 128 of them go through a tile together, with long, empty
+    and unused rows beside."""
+    lengths = [(37 * r) % 90 if r % 7 else -1 if r % 2 else 0 for r in range(rows)]
+    lengths[3], lengths[rows - 1] = 700, 1
+    b = ref.Batch(rows + dim, rows, kv_heads, group, dim, 16, prefix, lengths, io, cache)
+    d = Device(b)
+    out = d.attend(ctx, out=torch.full_like(d.q, 77.0))
+    check(b, out)
+    assert int(d.status) == 0 and all((out[r] == 77.0).all() for r, n in enumerate(lengths) if n < 0)
+
+
+@pytest.mark.parametrize("io,cache", [(F32, BF16), (BF16, F32)])
+def test_captured_calls_of_many_queries(ctx, io, cache):
+    b = ref.Batch(33, 40, 1, 16, 256, 16, 4999, [100] * 40, io, cache, junk=0.0)
+    d = Device(b)
+    ws = torch.empty(paged.attend_workspace(d.kv, d.rows, 16), dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(d.q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.attend(ctx, d.kv, d.rows, d.lengths, d.q, b.scale, out=out, workspace=ws)
+    gen = torch.Generator().manual_seed(9)
+    for step in range(4):
+        d.lengths.copy_(torch.randint(0, 101, (40,), generator=gen))
+        d.q.copy_(torch.randn(d.q.shape, generator=gen))
+        d.table.copy_(d.table[torch.randperm(40, generator=gen).cuda()])
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = paged.attend(ctx, d.kv, d.rows, d.lengths, d.q, b.scale)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager), step
+
+
 def test_threads_share_a_context(ctx):
     """Two threads, each with its stream, its batch and its logits."""
     cases, want = [], []

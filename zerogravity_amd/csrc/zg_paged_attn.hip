@@ -18,8 +18,7 @@
 //   O^T [element][query] += V^T P^T -- value rows are loaded 16 bytes a lane
 //     and transposed between a lane's own registers, 8 rows at a time (32-bit
 //     rows need not be).
-// So the tile needs neither LDS nor a barrier, and each key and value is read
-// from memory once per 16 MT queries.
+// So the tile needs neither LDS nor a barrier.
 #include <algorithm>
 #include <cmath>
 
@@ -29,7 +28,7 @@ namespace zg {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
-constexpr int kOwnWaves = 2048;     // waves over the rows' own tiles: two per SIMD
+constexpr int kOwnWaves = 1024;     // waves over the rows' own tiles: one per SIMD
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
 constexpr int kCus = 256;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -93,20 +92,17 @@ __device__ __forceinline__ void stage_queries(v4u* lds, int n, int thread, int t
     }
 }
 
-// A wave's running sums for 16 MT queries: lane l holds query l % 16 of each
-// tile; o[..][f][r] is element 16 W g + W (4 quarter + r) + i of it, f = W g + i.
-template <int D, int MT>
+// A wave's running sums for 16 queries: lane l holds query l % 16; o[f][r] is
+// element 16 W g + W (4 quarter + r) + i of it, f = W g + i.
+template <int D>
 struct Sums {
-    float ref[MT], l[MT];  // l: this lane's tokens only
-    v4f o[MT][D / 16];
+    float ref, l;  // l: this lane's tokens only
+    v4f o[D / 16];
     __device__ void clear() {
+        ref = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            ref[m] = -INFINITY;
-            l[m] = 0.0f;
-#pragma unroll
-            for (int f = 0; f < D / 16; ++f) o[m][f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        for (int f = 0; f < D / 16; ++f) o[f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
 };
 
@@ -132,27 +128,23 @@ __device__ __forceinline__ Place resolve(const PagedPool& p, uint32_t page, uint
 }
 
 // A tile's weights as operands of the second product.
-template <bool IO, bool KV, int D, int MT>
+template <bool IO, bool KV, int D>
 struct Weights {
     static constexpr int kParts = Form<IO, KV, D>::kWeightParts, kMine = Form<IO, KV, D>::kMine;
-    v4u part[MT][kParts];  // of bfloat16; a 32-bit cache takes the weights as they are
-    __device__ void operator=(const float (&w)[MT][kMine]) {
+    v4u part[kParts];  // of bfloat16; a 32-bit cache takes the weights as they are
+    __device__ void operator=(const float (&w)[kMine]) {
+        if constexpr (!KV) {
+            part[0] = v4u{__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3])};
+        } else {
+            float x[8];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if constexpr (!KV) {
-                part[m][0] = v4u{__float_as_uint(w[m][0]), __float_as_uint(w[m][1]), __float_as_uint(w[m][2]),
-                                 __float_as_uint(w[m][3])};
-            } else {
-                float x[8];
+            for (int j = 0; j < 8; ++j) x[j] = w[j];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = w[m][j];
+            for (int p = 0; p < kParts; ++p) {
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) {
+                for (int j = 0; j < 4; ++j) part[p][j] = pack_high(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) part[m][p][j] = pack_high(x[2 * j], x[2 * j + 1]);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] -= high_part(x[j]);
-                }
+                for (int j = 0; j < 8; ++j) x[j] -= high_part(x[j]);
             }
         }
     }
@@ -160,38 +152,36 @@ struct Weights {
 
 // A tile's weights e^(s - m) from its scores, m the query's reference: the
 // sums are brought to a new one only when a score passes the old one by
-// 2^kRaise, which 32-bit sums hold with ease.
-template <bool IO, bool KV, int D, int MT>
-__device__ __forceinline__ void weigh(const v4f (&sc)[MT][Form<IO, KV, D>::kHalves], uint32_t there, float to_log2,
-                                      int quarter, Sums<D, MT>& s, Weights<IO, KV, D, MT>& weights) {
+// 2^kRaise, which 32-bit sums hold with ease (64 rows over 32768 tokens 64 us;
+// with every higher score 69).
+template <bool IO, bool KV, int D>
+__device__ __forceinline__ void weigh(const v4f (&sc)[Form<IO, KV, D>::kHalves], uint32_t there, float to_log2,
+                                      int quarter, Sums<D>& s, Weights<IO, KV, D>& weights) {
     constexpr int N = Form<IO, KV, D>::kMine;
-    float w[MT][N];
+    float w[N];
     constexpr uint32_t kAll = N == 8 ? 0xffffffffu : 0xffffu;
+    float top = -INFINITY;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        float top = -INFINITY;
+    for (int j = 0; j < N; ++j) {
+        w[j] = Form<IO, KV, D>::kScaled ? sc[j >> 2][j & 3] : sc[j >> 2][j & 3] * to_log2;
+        if (there != kAll && !(there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u)) w[j] = -INFINITY;
+        top = fmaxf(top, w[j]);
+    }
+    top = fmaxf(top, other_quarter<16>(top));
+    top = fmaxf(top, other_quarter<32>(top));
+    if (__any(top > s.ref + kRaise)) {
+        const float to = fmaxf(top, s.ref);
+        const float keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.ref - to);
+        s.ref = to;
+        s.l *= keep;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            w[m][j] = Form<IO, KV, D>::kScaled ? sc[m][j >> 2][j & 3] : sc[m][j >> 2][j & 3] * to_log2;
-            if (there != kAll && !(there >> (16 * (j >> 2) + 4 * quarter + (j & 3)) & 1u)) w[m][j] = -INFINITY;
-            top = fmaxf(top, w[m][j]);
-        }
-        top = fmaxf(top, other_quarter<16>(top));
-        top = fmaxf(top, other_quarter<32>(top));
-        if (__any(top > s.ref[m] + kRaise)) {
-            const float to = fmaxf(top, s.ref[m]);
-            const float keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.ref[m] - to);
-            s.ref[m] = to;
-            s.l[m] *= keep;
+        for (int f = 0; f < D / 16; ++f) s.o[f] *= keep;
+    }
+    const float sub = s.ref == -INFINITY ? 0.0f : s.ref;
 #pragma unroll
-            for (int f = 0; f < D / 16; ++f) s.o[m][f] *= keep;
-        }
-        const float sub = s.ref[m] == -INFINITY ? 0.0f : s.ref[m];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            w[m][j] = __builtin_amdgcn_exp2f(w[m][j] - sub);
-            s.l[m] += w[m][j];
-        }
+    for (int j = 0; j < N; ++j) {
+        w[j] = __builtin_amdgcn_exp2f(w[j] - sub);
+        s.l += w[j];
     }
     weights = w;
 }
@@ -209,9 +199,8 @@ __device__ __forceinline__ void drop_values(uint32_t (&v)[N][VR], uint32_t there
 }
 
 // One load's worth of a tile's value rows, weighted, added to the sums.
-template <bool IO, bool KV, int D, int MT, int N, int VR>
-__device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const Weights<IO, KV, D, MT>& w, int g,
-                                           Sums<D, MT>& s) {
+template <bool IO, bool KV, int D, int N, int VR>
+__device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const Weights<IO, KV, D>& w, int g, Sums<D>& s) {
     using F = Form<IO, KV, D>;
     constexpr int W = F::kWide;
     if constexpr (KV) {
@@ -229,29 +218,24 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const Wei
 #pragma unroll
             for (int p = 0; p < F::kWeightParts; ++p)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                        s.o[m][g * W + from + i] = mfma_bf16(rows[i], w.part[m][p], s.o[m][g * W + from + i]);
+                for (int i = 0; i < 2; ++i) s.o[g * W + from + i] = mfma_bf16(rows[i], w.part[p], s.o[g * W + from + i]);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
 #pragma unroll
             for (int i = 0; i < W; ++i)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    s.o[m][g * W + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                        __uint_as_float(v[j][i]), __uint_as_float(w.part[m][0][j]), s.o[m][g * W + i], 0, 0, 0);
+                s.o[g * W + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][i]),
+                                                                      __uint_as_float(w.part[0][j]), s.o[g * W + i], 0, 0, 0);
     }
 }
 
 // Tiles tile, tile + step, ... before `end` of one table added to the sums;
 // page is what the table says of the first.
-template <bool IO, bool KV, int D, int MT>
+template <bool IO, bool KV, int D>
 __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* queries, int n, const int32_t* table,
                                           uint32_t tokens, int tile, int end, int step, int kvh, uint32_t page,
-                                          Sums<D, MT>& s, int& bad) {
+                                          Sums<D>& s, int& bad) {
     using F = Form<IO, KV, D>;
     constexpr int W = F::kWide, H = F::kHalves, N = F::kMine;
     constexpr int ES = KV ? 2 : 4, VR = W * ES / 4;  // registers of a value row per load
@@ -300,47 +284,43 @@ __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* que
         page = peek<F::kTile>(a.pool, table, tokens, tile + step, lane);
         __builtin_amdgcn_sched_barrier(0);
         // scores
-        v4f sc[MT][H];
+        v4f sc[H];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < H; ++h) sc[m][h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < H; ++h) sc[h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         // the queries' places are stepped through: kept for all steps they
         // would take the registers of a quarter of the keys
-        int place = quarter * n + (MT == 1 ? min(col, n - 1) : col);
+        int place = quarter * n + min(col, n - 1);
         asm volatile("" : "+v"(place));
 #pragma unroll
         for (int i = 0; i < F::kSteps; ++i) {
 #pragma unroll
-            for (int p = 0; p < F::kParts; ++p, place += 4 * n)
+            for (int p = 0; p < F::kParts; ++p, place += 4 * n) {
+                const v4u b = queries[place];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const v4u b = queries[place + 16 * m];
+                for (int h = 0; h < H; ++h) {
+                    if constexpr (KV) {
+                        sc[h] = mfma_bf16(k[h][i], b, sc[h]);
+                    } else {
 #pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        if constexpr (KV) {
-                            sc[m][h] = mfma_bf16(k[h][i], b, sc[m][h]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                sc[m][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    __uint_as_float(k[h][i][e]), __uint_as_float(b[e]), sc[m][h], 0, 0, 0);
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h][i][e]), __uint_as_float(b[e]),
+                                                                         sc[h], 0, 0, 0);
                     }
                 }
+            }
             // two steps' queries in registers at a time
             if (i & 1) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int g = kFirst; g < F::kLoads; ++g) load_values(g);
         __builtin_amdgcn_sched_barrier(0);
-        Weights<IO, KV, D, MT> w;
-        weigh<IO, KV, D, MT>(sc, there, to_log2, quarter, s, w);
+        Weights<IO, KV, D> w;
+        weigh<IO, KV, D>(sc, there, to_log2, quarter, s, w);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < F::kLoads; ++g) {
             drop_values<KV>(v[g], there, quarter);
-            add_values<IO, KV, D, MT>(v[g], w, g, s);
+            add_values<IO, KV, D>(v[g], w, g, s);
         }
     }
 }
@@ -360,53 +340,42 @@ __device__ __forceinline__ void store_sums(float2* stats, float* o, int across, 
 
 // The sums of waves 0 .. n - 1 brought together in wave 0, in a fixed order;
 // every wave of the workgroup calls this.
-template <int D, int MT>
-__device__ __forceinline__ void gather_waves(Sums<D, MT>& s, int n, int wave, int lane, char* lds) {
+template <int D>
+__device__ __forceinline__ void gather_waves(Sums<D>& s, int n, int wave, int lane, char* lds) {
     const int quarter = lane >> 4, col = lane & 15;
-    float2* stats = (float2*)lds;  // [n][16 MT]
-    v4f* part = (v4f*)(lds + n * 16 * MT * sizeof(float2));
-    const bool mine = wave < n;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        s.l[m] += __shfl_xor(s.l[m], 16, kWave);
-        s.l[m] += __shfl_xor(s.l[m], 32, kWave);
-        if (mine && quarter == 0) stats[wave * 16 * MT + 16 * m + col] = make_float2(s.ref[m], s.l[m]);
-    }
+    float2* stats = (float2*)lds;  // [n][16]
+    v4f* part = (v4f*)(lds + n * 16 * sizeof(float2));
+    s.l += __shfl_xor(s.l, 16, kWave);
+    s.l += __shfl_xor(s.l, 32, kWave);
+    if (wave < n && quarter == 0) stats[wave * 16 + col] = make_float2(s.ref, s.l);
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        float top = -INFINITY;
-        for (int w = 0; w < n; ++w) top = fmaxf(top, stats[w * 16 * MT + 16 * m + col].x);
-        const float sub = top == -INFINITY ? 0.0f : top;
-        s.l[m] = 0.0f;
-        for (int w = 0; w < n; ++w) {
-            const float2 x = stats[w * 16 * MT + 16 * m + col];
-            s.l[m] += x.y * __builtin_amdgcn_exp2f(x.x == top ? 0.0f : x.x - sub);
-        }
-        const float keep = __builtin_amdgcn_exp2f(s.ref[m] == top ? 0.0f : s.ref[m] - sub);
-        s.ref[m] = top;
-#pragma unroll
-        for (int f = 0; f < D / 16; ++f) s.o[m][f] *= keep;
+    float top = -INFINITY;
+    for (int w = 0; w < n; ++w) top = fmaxf(top, stats[w * 16 + col].x);
+    const float sub = top == -INFINITY ? 0.0f : top;
+    s.l = 0.0f;
+    for (int w = 0; w < n; ++w) {
+        const float2 x = stats[w * 16 + col];
+        s.l += x.y * __builtin_amdgcn_exp2f(x.x == top ? 0.0f : x.x - sub);
     }
+    const float keep = __builtin_amdgcn_exp2f(s.ref == top ? 0.0f : s.ref - sub);
+    s.ref = top;
+#pragma unroll
+    for (int f = 0; f < D / 16; ++f) s.o[f] *= keep;
     while (n > 1) {
         const int half = (n + 1) / 2;
         if (wave >= half && wave < n)
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int f = 0; f < D / 16; ++f) part[(((wave - half) * MT + m) * (D / 16) + f) * 64 + lane] = s.o[m][f];
+            for (int f = 0; f < D / 16; ++f) part[((wave - half) * (D / 16) + f) * 64 + lane] = s.o[f];
         __syncthreads();
         if (wave < n - half)
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int f = 0; f < D / 16; ++f) s.o[m][f] += part[((wave * MT + m) * (D / 16) + f) * 64 + lane];
+            for (int f = 0; f < D / 16; ++f) s.o[f] += part[(wave * (D / 16) + f) * 64 + lane];
         __syncthreads();
         n = half;
     }
 }
-constexpr size_t gather_bytes(int waves, int mt, int head_dim) {
-    return (size_t)waves * 16 * mt * sizeof(float2) + (size_t)(waves / 2) * mt * head_dim * 64;
+constexpr size_t gather_bytes(int waves, int head_dim) {
+    return (size_t)waves * 16 * sizeof(float2) + (size_t)(waves / 2) * head_dim * 64;
 }
 
 // How a call is cut.  The prefix: `chunks` pieces of chunk_tiles tiles, each
@@ -495,7 +464,7 @@ __device__ __forceinline__ PieceOf piece_of(const Cut& c, int kv_heads, int id) 
     return p;
 }
 
-template <bool IO, bool KV, int D, int MT>
+template <bool IO, bool KV, int D>
 __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
     const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -510,23 +479,21 @@ __device__ __forceinline__ void prefix_block(const PagedAttnArgs& a, const Cut& 
             const int f = min(first + m, last), r = f / a.group;
             return r * a.q_stride + (size_t)(kvh * a.group + f - r * a.group) * D;
         }
-    } who{a.q, a, block * 16 * MT, queries - 1, kvh};
+    } who{a.q, a, block * 16, queries - 1, kvh};
     const int first = chunk * c.chunk_tiles;
     const uint32_t page = peek<Form<IO, KV, D>::kTile>(a.pool, a.prefix, a.prefix_tokens, first + wave, lane);
-    stage_queries<IO, KV, D>((v4u*)lds, 16 * MT, tid, 256, a.scale * kLog2e, who);
+    stage_queries<IO, KV, D>((v4u*)lds, 16, tid, 256, a.scale * kLog2e, who);
     __syncthreads();
-    Sums<D, MT> s;
+    Sums<D> s;
     s.clear();
     int bad = 0;
-    add_tiles<IO, KV, D, MT>(a, (const v4u*)lds, 16 * MT, a.prefix, a.prefix_tokens, first + wave,
-                             min(first + c.chunk_tiles, c.prefix_tiles), 4, kvh, page, s, bad);
+    add_tiles<IO, KV, D>(a, (const v4u*)lds, 16, a.prefix, a.prefix_tokens, first + wave,
+                         min(first + c.chunk_tiles, c.prefix_tiles), 4, kvh, page, s, bad);
     if (bad && a.status) atomicOr(a.status, bad);
     __syncthreads();
-    gather_waves<D, MT>(s, 4, wave, lane, lds);
+    gather_waves<D>(s, 4, wave, lane, lds);
     if (wave) return;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-        store_prefix<D>(a, c, kvh * c.chunks + chunk, block * 16 * MT + 16 * m + col, s.o[m], s.ref[m], s.l[m], quarter);
+    store_prefix<D>(a, c, kvh * c.chunks + chunk, block * 16 + col, s.o, s.ref, s.l, quarter);
 }
 
 // LDS of own_block's table: 68 words for each wave, or one for all of them.
@@ -612,7 +579,7 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
     const bool gathered = upto - from <= tiles - in_first % tiles;
     v4u* queries = (v4u*)(lds + table_bytes(a.rows, WAVES)) + wave * F::kParts * F::kSteps * 4 * a.group;
     bad = 0;
-    Sums<D, 1> s;
+    Sums<D> s;
     s.clear();
     while (t < end) {
         const uint32_t before = at_row(r), n = at_row(r + 1) - before;
@@ -631,35 +598,35 @@ __device__ __forceinline__ void own_block(const PagedAttnArgs& a, const Cut& c, 
         const uint32_t here = own_tokens(a, r), page = peek<F::kTile>(a.pool, table, here, (int)tile, lane);
         stage_queries<IO, KV, D>(queries, a.group, lane, 64, a.scale * kLog2e, who);
         same_wave();
-        add_tiles<IO, KV, D, 1>(a, queries, a.group, table, here, (int)tile, (int)upto_tile, 1, (int)kvh, page, s, bad);
+        add_tiles<IO, KV, D>(a, queries, a.group, table, here, (int)tile, (int)upto_tile, 1, (int)kvh, page, s, bad);
         same_wave();
         t += upto_tile - tile;
         if (gathered) break;
-        s.l[0] += __shfl_xor(s.l[0], 16, kWave);
-        s.l[0] += __shfl_xor(s.l[0], 32, kWave);
+        s.l += __shfl_xor(s.l, 16, kWave);
+        s.l += __shfl_xor(s.l, 32, kWave);
         const size_t piece = (size_t)w + r * kvs + kvh;
         if (col < a.group)
-            store_sums<D>(c.own_stats + piece * a.group, c.own_o + piece * a.group * D, a.group, col, s.o[0], s.ref[0],
-                          s.l[0], quarter);
+            store_sums<D>(c.own_stats + piece * a.group, c.own_o + piece * a.group * D, a.group, col, s.o, s.ref,
+                          s.l, quarter);
         s.clear();
     }
     if (bad && a.status) atomicOr(a.status, bad);
     if (!gathered) return;
     __syncthreads();
-    gather_waves<D, 1>(s, share.active, wave, lane, lds);
+    gather_waves<D>(s, share.active, wave, lane, lds);
     const size_t piece = (size_t)w + r * kvs + in_first / tiles;
     if (wave == 0 && col < a.group)
-        store_sums<D>(c.own_stats + piece * a.group, c.own_o + piece * a.group * D, a.group, col, s.o[0], s.ref[0], s.l[0],
+        store_sums<D>(c.own_stats + piece * a.group, c.own_o + piece * a.group * D, a.group, col, s.o, s.ref, s.l,
                       quarter);
 }
 
-// Few queries over the prefix (16 MT a pass): it is bound by memory, so the
-// four waves take tiles of their own, straight into registers.
-template <bool IO, bool KV, int D, int MT>
-__global__ __launch_bounds__(256, MT * D > 256 ? 1 : 2) void paged_attn_kernel(PagedAttnArgs a, Cut c) {
+// Over the prefix 16 queries a workgroup, whose four waves take tiles of their
+// own, straight into registers.
+template <bool IO, bool KV, int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, Cut c) {
     extern __shared__ __align__(16) char lds[];
     const int over_prefix = c.chunks * c.blocks * a.pool.kv_heads;
-    if ((int)blockIdx.x < over_prefix) prefix_block<IO, KV, D, MT>(a, c, blockIdx.x, lds);
+    if ((int)blockIdx.x < over_prefix) prefix_block<IO, KV, D>(a, c, blockIdx.x, lds);
     else own_block<IO, KV, D, 4>(a, c, blockIdx.x - over_prefix, lds);
 }
 
@@ -783,9 +750,9 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
             }
         }
     }
-    Sums<D, 1> s;
+    Sums<D> s;
     s.clear();
-    Weights<IO, KV, D, 1> w;
+    Weights<IO, KV, D> w;
     uint32_t v[N][VR];
     auto load_values = [&](int g, int buffer) {
         const char* const data = lds + buffer * 2 * kHalf;
@@ -811,7 +778,7 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
         for (int g = 0; g < F::kLoads; ++g) {
             if (g) load_values(g, buffer);
             drop_values<KV>(v, there, quarter);
-            add_values<IO, KV, D, 1>(v, w, g, s);
+            add_values<IO, KV, D>(v, w, g, s);
         }
     };
     // Two tiles between barriers: within them the two waves of a SIMD drift
@@ -851,9 +818,9 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
         };
         load_keys(0);
         if (F::kSteps > 1) load_keys(1);
-        v4f sc[1][H];
+        v4f sc[H];
 #pragma unroll
-        for (int h = 0; h < H; ++h) sc[0][h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < H; ++h) sc[h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < F::kSteps; ++i) {
             if (i + 2 < F::kSteps) load_keys(i + 2);
@@ -863,12 +830,12 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     if constexpr (KV) {
-                        sc[0][h] = mfma_bf16(k[i % 3][h], q[p][i], sc[0][h]);
+                        sc[h] = mfma_bf16(k[i % 3][h], q[p][i], sc[h]);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            sc[0][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i % 3][h][e]),
-                                                                            __uint_as_float(q[0][i][e]), sc[0][h], 0, 0, 0);
+                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i % 3][h][e]),
+                                                                            __uint_as_float(q[0][i][e]), sc[h], 0, 0, 0);
                     }
                 }
             __builtin_amdgcn_sched_barrier(0);
@@ -876,15 +843,15 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c,
         load_values(0, buffer);
         if (half == 0) fetch(local + 2, pair ^ 2);
         __builtin_amdgcn_sched_barrier(0);
-        weigh<IO, KV, D, 1>(sc, there[half], to_log2, quarter, s, w);
+        weigh<IO, KV, D>(sc, there[half], to_log2, quarter, s, w);
         add(there[half], buffer);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's LDS
     if (bad && a.status) atomicOr(a.status, bad);
-    s.l[0] += __shfl_xor(s.l[0], 16, kWave);
-    s.l[0] += __shfl_xor(s.l[0], 32, kWave);
-    store_prefix<D>(a, c, kvh * c.chunks + at_piece.chunk, mine, s.o[0], s.ref[0], s.l[0], quarter);
+    s.l += __shfl_xor(s.l, 16, kWave);
+    s.l += __shfl_xor(s.l, 32, kWave);
+    store_prefix<D>(a, c, kvh * c.chunks + at_piece.chunk, mine, s.o, s.ref, s.l, quarter);
 }
 
 template <bool IO, bool KV, int D>
@@ -989,20 +956,28 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnArgs a, Cu
 
 // ------------------------------------------------------------------- host
 
-// Queries of one kv head that go over the prefix in one pass: 16 or 32 in a
-// wave, or 128 in a workgroup.
-static int block_of(uint32_t rows, int group) {
-    const uint64_t n = (uint64_t)rows * group;
-    return n <= 16 ? 16 : n <= 32 ? 32 : kManyQueries;
+// Queries of one kv head that go over a tile of the prefix together: 16, in one
+// wave, or 128, in a workgroup that reads the tile for all of them.  The
+// latter is slow to start and leaves larger pieces, so it takes over where 16
+// at a time would give each of 1024 waves more than 6 tiles.  256-element heads,
+// 8 queries a row on 2 kv heads, both launches, 16 at a time and 128: 32 rows
+// over 512 tokens 13.4 and 18.0 us, over 2048 16.4 and 21.4, over 8192 (4 tiles
+// a wave) 24.2 and 31.0, over 16384 (8) 35.3 and 39.1, 16-bit queries 32.5 and
+// 32.0, over 32768 57.0 and 53.7 (51.9, 43.2); 16 rows over 32768 (8) 36.0 and
+// 36.9 (33.9, 30.1); 128-element heads, 24 rows over 2048 (2) 13.6 and 15.6,
+// 32 over 8192 (10) 28.2 and 28.8.
+constexpr uint64_t kFewTiles = 6 * 1024;
+static int block_of(uint64_t queries, int kv_heads, uint64_t tiles) {
+    return queries <= 16 || (queries + 15) / 16 * kv_heads * tiles <= kFewTiles ? 16 : kManyQueries;
 }
 
 static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int tile, uint32_t prefix_tokens,
                   uint64_t row_tokens, size_t query_bytes, void* workspace, size_t* bytes) {
     Cut c{};
     const int group = q_heads / kv_heads;
-    c.block = block_of(rows, group);
-    c.blocks = (int)(((uint64_t)rows * group + c.block - 1) / c.block);
     c.prefix_tiles = (int)((prefix_tokens + tile - 1) / tile);
+    c.block = block_of((uint64_t)rows * group, kv_heads, c.prefix_tiles);
+    c.blocks = (int)(((uint64_t)rows * group + c.block - 1) / c.block);
     if (c.prefix_tiles) {
         // More pieces run side by side, and each costs the join: with T tiles
         // in all, a tile taking some 2 us and a piece of 128 queries adding
@@ -1072,14 +1047,12 @@ static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
     const bool many = c.chunks && c.block == kManyQueries;
     const int waves = many ? kManyWaves : 4;
     constexpr size_t query = query_bytes<IO, KV, D>();
-    const size_t own = std::max(table_bytes(a.rows, waves) + c.per_group * a.group * query, gather_bytes(c.per_group, 1, D));
+    const size_t own = std::max(table_bytes(a.rows, waves) + c.per_group * a.group * query, gather_bytes(c.per_group, D));
     size_t prefix = 0;
     if (many) prefix = (size_t)kBuffers * 2 * F::kTile * D * (KV ? 2 : 4) + (size_t)kSegment * F::kTile * 4;
-    else if (c.chunks) prefix = std::max(query * c.block, gather_bytes(4, c.block / 16, D));
+    else if (c.chunks) prefix = std::max(query * c.block, gather_bytes(4, D));
     const size_t lds = std::max(prefix, own);
-    void (*kernel)(PagedAttnArgs, Cut) = many                            ? paged_attn_many_kernel<IO, KV, D>
-                                         : c.chunks && c.block == 32 ? paged_attn_kernel<IO, KV, D, 2>
-                                                                         : paged_attn_kernel<IO, KV, D, 1>;
+    void (*kernel)(PagedAttnArgs, Cut) = many ? paged_attn_many_kernel<IO, KV, D> : paged_attn_kernel<IO, KV, D>;
     if (lds > 65536) {
         hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
