@@ -11,6 +11,13 @@
 // takes them a lane each.  The count of a token is a sum of integers and the
 // list's order of no account, so the order of the LDS atomics does not matter;
 // the biases of one token are summed in their order.
+//
+// The bytes of 32 rows of 151936 take 7.7 us, a copy through this kernel with a
+// mask 11.4; 500 tokens of history make it 16 us and 2500 17: barriers and
+// shared memory between a slice's loads and its stores, and 1216 workgroups
+// where 1024 run at once.  With 64 rows of 9000 tokens 29 us: the histories,
+// 38 slices of each row reading them from the L2s, are then 88 MB beside the
+// logits' 39.
 #include "zg_paged.hpp"
 
 namespace zg {

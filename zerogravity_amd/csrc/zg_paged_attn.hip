@@ -28,7 +28,12 @@ namespace zg {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
-constexpr int kOwnWaves = 1024;     // waves over the rows' own tiles: one per SIMD
+// Waves over the rows' own tiles: one per SIMD, since a tile's loads are all under
+// way at once (8 rows of 32768 tokens 101 us = 5.3 TB/s) and every wave leaves
+// pieces to join.  With 2048 one row of 32768 took 18.1 + 8.9 us for 17.4 + 6.2,
+// 24 rows of up to 16384 24.4 + 7.2 for 22.3 + 5.7, 32 of up to 4096 with
+// 64-element heads 47.4 for 43.6, only 200 short rows of those 35.7 for 40.5.
+constexpr int kOwnWaves = 1024;
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
 constexpr int kCus = 256;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -231,7 +236,10 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[N][VR], const Wei
 }
 
 // Tiles tile, tile + step, ... before `end` of one table added to the sums;
-// page is what the table says of the first.
+// page is what the table says of the first.  Bound by memory where the tiles
+// are read once (5.3 TB/s of a bfloat16 cache, 5.6 of a 32-bit one), by the
+// chain of a tile's loads and products where a wave has few: one row of 2048
+// tokens, a tile to a wave, 7.6 us.
 template <bool IO, bool KV, int D>
 __device__ __forceinline__ void add_tiles(const PagedAttnArgs& a, const v4u* queries, int n, const int32_t* table,
                                           uint32_t tokens, int tile, int end, int step, int kvh, uint32_t page,
@@ -636,9 +644,18 @@ constexpr int kSegment = 64;                        // tiles looked up at a time
 
 // Many queries over the prefix: each of eight waves holds 16 queries and their
 // sums in registers, and all go through the same tiles, which are copied
-// straight to LDS three tiles ahead; a tile is read from memory once for 128
-// queries.  In LDS the 16-byte pieces of row t are exchanged by an xor of t,
-// so that 16 lanes reading one piece of 16 rows meet 16 different banks.
+// straight to LDS, two in use and two coming; a tile is read from memory once
+// for 128 queries.  In LDS the 16-byte pieces of row t are exchanged by an xor of
+// t, so that 16 lanes reading one piece of 16 rows meet 16 different banks.
+// Bound by the matrix cores and what stands between their products: 64 rows
+// over 32768 tokens (256-element heads) 64 us, 52 GFLOP of three-part bfloat16
+// products = 0.8 PFLOP/s where a large library product reaches 1.1, with 16-bit
+// queries 49 us; 44 MB are fetched for the cache's 34.  Of a pair of tiles the
+// scores take 1800 cycles (1536 of them products), the values 2420 (1536, and 64
+// byte permutations that transpose them), weights and copies the rest.  Each
+// query's registers fill the file, so a SIMD holds two waves; copies placed
+// elsewhere between the products, another priority in them, or half the waves
+// a phase later took as long or longer.
 template <bool IO, bool KV, int D>
 __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
     using F = Form<IO, KV, D>;
@@ -871,7 +888,10 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_attn_many_kernel(Pag
 
 // Workgroup (kv head, row, four accumulators): a thread owns 16 bytes of the
 // pieces, (accumulator, quarter, query), and every n-th piece; the n threads
-// of one item are joined at the end, in order.
+// of one item are joined at the end, in order.  Pieces lie in the order of the
+// sums, so that neighbouring threads read whole lines: 64 rows, 64 pieces each
+// for a head, 34 MB, take 10 us.  A few pieces are a launch, the look at `runs`
+// and two rounds of loads: 4 to 5 us.
 template <bool IO, int D, int W, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnArgs a, Cut c) {
     constexpr int kJoin = THREADS == 1024 ? 4 : 8;  // pieces that a thread has under way
@@ -981,12 +1001,12 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
     if (c.prefix_tiles) {
         // More pieces run side by side, and each costs the join: with T tiles
         // in all, a tile taking some 2 us and a piece of 128 queries adding
-        // 0.1 us (256-element heads), sqrt(20 T) pieces.  32 rows over 8192
-        // tokens: 256 pieces 25 + 12 us, 128 pieces 21 + 8; over 2048: 64
-        // pieces 15 + 6, 32 pieces 19 + 4.  A piece of few queries is cheap: one
-        // tile for each wave.
+        // 0.05 us (256-element heads), sqrt(40 T) pieces.  32 rows over 16384
+        // tokens: 256 pieces 31 + 9 us, 172 pieces 28 + 8, 128 pieces 31 + 8,
+        // 104 pieces 36 + 6.  A piece of few queries is cheap: one tile for each
+        // wave, up to a piece to a CU (two: 32 rows over 8192 23 + 6, one 20 + 4).
         const int share = kv_heads * c.blocks;
-        const int most = c.block == kManyQueries ? (int)std::sqrt(20.0 * c.prefix_tiles * share) / share
+        const int most = c.block == kManyQueries ? (int)std::sqrt(40.0 * c.prefix_tiles * share) / share
                                                  : std::min((c.prefix_tiles + 3) / 4, kCus / share);
         const int want = std::max(1, std::min({most, c.prefix_tiles, kCus / share}));
         c.chunk_tiles = (c.prefix_tiles + want - 1) / want;
@@ -1003,7 +1023,8 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
     const uint64_t own_tiles = (uint64_t)rows * kv_heads * ((row_tokens + tile - 1) / tile);
     int most = kOwnWaves / c.per_group;
     if (many) {
-        // the CUs that the prefix leaves, if they are a quarter of them
+        // the CUs that the prefix leaves, if they are a quarter of them (32 rows
+        // with 2048 tokens of their own over 16384: 32 us, spread over all 39)
         const int left = kCus - c.chunks * c.blocks * kv_heads;
         most = left >= kCus / 4 ? left : kCus;
     }
