@@ -650,12 +650,12 @@ constexpr int kSegment = 64;                        // tiles looked up at a time
 // Bound by the matrix cores and what stands between their products: 64 rows
 // over 32768 tokens (256-element heads) 64 us, 52 GFLOP of three-part bfloat16
 // products = 0.8 PFLOP/s where a large library product reaches 1.1, with 16-bit
-// queries 49 us; 44 MB are fetched for the cache's 34.  Of a pair of tiles the
-// scores take 1800 cycles (1536 of them products), the values 2420 (1536, and 64
-// byte permutations that transpose them), weights and copies the rest.  Each
-// query's registers fill the file, so a SIMD holds two waves; copies placed
-// elsewhere between the products, another priority in them, or half the waves
-// a phase later took as long or longer.
+// queries 49 us; with own tokens 91 MB are fetched of 88 there are.  Of a pair
+// of tiles the scores take 1800 cycles (1536 of them products), the values 2420
+// (1536, and 64 byte permutations that transpose them), weights and copies the
+// rest.  16 queries and their sums fill a wave's registers, so a SIMD holds two
+// waves; copies placed elsewhere between the products, another priority in
+// them, or half the waves a phase later took as long or longer.
 template <bool IO, bool KV, int D>
 __device__ __forceinline__ void many_block(const PagedAttnArgs& a, const Cut& c, int id, char* lds) {
     using F = Form<IO, KV, D>;
@@ -981,11 +981,11 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnArgs a, Cu
 // latter is slow to start and leaves larger pieces, so it takes over where 16
 // at a time would give each of 1024 waves more than 6 tiles.  256-element heads,
 // 8 queries a row on 2 kv heads, both launches, 16 at a time and 128: 32 rows
-// over 512 tokens 13.4 and 18.0 us, over 2048 16.4 and 21.4, over 8192 (4 tiles
-// a wave) 24.2 and 31.0, over 16384 (8) 35.3 and 39.1, 16-bit queries 32.5 and
-// 32.0, over 32768 57.0 and 53.7 (51.9, 43.2); 16 rows over 32768 (8) 36.0 and
-// 36.9 (33.9, 30.1); 128-element heads, 24 rows over 2048 (2) 13.6 and 15.6,
-// 32 over 8192 (10) 28.2 and 28.8.
+// over 512 tokens 13.5 and 17.9 us, over 2048 16.6 and 21.4, over 8192 (4 tiles
+// a wave) 23.6 and 29.7, over 16384 (8) 35.0 and 35.5, over 32768 57.0 and 52.0;
+// 16-bit queries there 21.9 and 24.8, 32.1 and 29.3, 51.9 and 42.0; 16 rows over
+// 32768 (8) 36.2 and 39.4; 128-element heads, 64 rows over 2048 (5) 19.6 and
+// 17.4, 32 over 8192 (10) 27.9 and 26.3.
 constexpr uint64_t kFewTiles = 6 * 1024;
 static int block_of(uint64_t queries, int kv_heads, uint64_t tiles) {
     return queries <= 16 || (queries + 15) / 16 * kv_heads * tiles <= kFewTiles ? 16 : kManyQueries;
