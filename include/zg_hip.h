@@ -615,7 +615,7 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
 
 /* Attention of one query token per row over the shared prefix and the row's
  * own lengths[r] tokens (device, [rows->rows]), on the caller's stream; the
- * prefix's keys and values are read once for the whole batch.  out[r][h] =
+ * prefix's keys and values are read for many rows together.  out[r][h] =
  * sum_t e^(scale q.k_t - m) v_t / sum_t e^(scale q.k_t - m) with kv head h /
  * (q_heads / kv_heads), the softmax of lib.rs:1352-1387 and the value sum of
  * lib.rs:1276-1305 regrouped: sums in 32 bits; 32-bit queries enter the
@@ -633,9 +633,10 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
  * pool are left out (ZG_STATUS_PAGE).  What slots past a row's length hold
  * does not matter.  NaN and infinities among the tokens come through as the
  * formula has them, but that an infinite key or value of a ZG_BF16 cache
- * may make what it enters NaN (the parts of a 32-bit factor can be 0).
- * |scale| below 2^127.  workspace of zg_paged_attn_workspace_bytes bytes (0 for
- * arguments that the call refuses), 16-byte aligned, is written and read by
+ * may make what it enters NaN (the parts of a 32-bit factor can be 0).  A
+ * query whose scores are all -inf gets zeros.  |scale| below 2^127.  workspace of zg_paged_attn_workspace_bytes bytes (0 for
+ * arguments that the call refuses; as many serve any call with no more rows,
+ * tokens a row can hold and prefix tokens), 16-byte aligned, is written and read by
  * the call: calls, and replays of captured ones, that may run at the same
  * time need one each.  A captured call keeps prefix_tokens and the pointers,
  * and reads the tables and lengths anew at each replay.  Asynchronous. */

@@ -147,3 +147,18 @@ def test_streams_of_another_device_are_refused():
     assert _torch.stream_of(ctx, here) is here
     with pytest.raises(L.ZgError):
         _torch.stream_of(ctx, SimpleNamespace(device=torch.device("cuda", 1)))
+
+
+def test_workspace_of_a_larger_batch_serves_smaller_ones():
+    rng = np.random.default_rng(3)
+    lib = L.lib()
+    for heads, q, dim, dtype in ((2, 8, 256, torch.bfloat16), (4, 20, 128, torch.float32), (8, 8, 64, torch.bfloat16)):
+        kv = pool(heads=heads, dim=dim, dtype=dtype)
+
+        def need(rows, stride, prefix):
+            return lib.zg_paged_attn_workspace_bytes(kv, L.PagedRows(4096, rows, stride, 4096, prefix), q)
+
+        for rows, stride, prefix in rng.integers(1, (200, 3000, 70000), (100, 3)):
+            most = need(rows, stride, prefix)
+            for part in rng.random((20, 3)):
+                assert need(max(1, int(rows * part[0])), max(1, int(stride * part[1])), int(prefix * part[2])) <= most

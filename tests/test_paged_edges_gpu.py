@@ -51,6 +51,24 @@ def test_sixteen_query_heads_over_a_prefix(ctx, io, cache):
     check(b, Device(b).attend(ctx))
 
 
+@pytest.mark.parametrize("io,cache", TYPES)
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_sixteen_query_heads_of_many_rows(ctx, io, cache, prefix):
+    lengths = [(41 * r) % 70 for r in range(70)]
+    b = ref.Batch(34, 70, 1, 16, 256, 8, prefix, lengths, io, cache)
+    check(b, Device(b).attend(ctx))
+
+
+def test_scores_that_are_all_minus_infinity_give_zeros(ctx):
+    b = ref.Batch(35, 3, 1, 1, 64, 16, 0, [20, 20, 1], F32, F32, junk=0.0)
+    for r, n in ((0, 20), (2, 1)):
+        i = torch.arange(n)
+        b.keys[b.table[r].long()[i // 16], i % 16, 0] = -torch.inf * b.q[r, 0].sign()
+    out = Device(b).attend(ctx)
+    assert (out[0] == 0).all() and (out[2] == 0).all()
+    check_row(b, out, 1)
+
+
 @pytest.mark.parametrize("io,cache", [(F32, BF16), (BF16, F32)])
 def test_captured_calls_over_a_prefix(ctx, io, cache):
     """Many queries over the prefix: replays follow lengths, tables and
@@ -108,6 +126,23 @@ def test_captured_calls_of_many_queries(ctx, io, cache):
         eager = paged.attend(ctx, d.kv, d.rows, d.lengths, d.q, b.scale)
         torch.cuda.synchronize()
         assert torch.equal(out, eager), step
+
+
+@pytest.mark.parametrize("rows,group,prefix", [(1, 4, 700), (4, 4, 700), (5, 4, 5000), (17, 16, 5000), (30, 16, 5000),
+                                               (40, 16, 5000), (40, 16, 0), (40, 1, 31)])
+@pytest.mark.parametrize("io,cache", TYPES)
+def test_calls_stay_inside_their_workspace(ctx, io, cache, rows, group, prefix):
+    """What the largest batch's workspace is sized for serves each of these, and
+    nothing behind it changes."""
+    b = ref.Batch(rows, rows, 2, group, 64, 16, prefix, [(29 * r) % 50 for r in range(rows)], io, cache, wide=4)
+    d = Device(b)
+    most = L.lib().zg_paged_attn_workspace_bytes(d.kv, L.PagedRows(4096, 40, 4, 4096, 5000), 2 * group)
+    need = paged.attend_workspace(d.kv, d.rows, 2 * group)
+    assert need <= most
+    for n in (need, most):
+        ws = torch.full((most + 65536,), 165, dtype=torch.uint8, device="cuda")
+        check(b, d.attend(ctx, workspace=ws[:n]))
+        assert (ws[n:] == 165).all()
 
 
 def test_threads_share_a_context(ctx):

@@ -28,14 +28,15 @@ namespace zg {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
+constexpr int kCus = 256;
 // Waves over the rows' own tiles: one per SIMD, since a tile's loads are all under
 // way at once (8 rows of 32768 tokens 101 us = 5.3 TB/s) and every wave leaves
 // pieces to join.  With 2048 one row of 32768 took 18.1 + 8.9 us for 17.4 + 6.2,
 // 24 rows of up to 16384 24.4 + 7.2 for 22.3 + 5.7, 32 of up to 4096 with
 // 64-element heads 47.4 for 43.6, only 200 short rows of those 35.7 for 40.5.
 constexpr int kOwnWaves = 1024;
+static_assert(kOwnWaves <= 4 * kCus, "paged_attn_workspace counts a workgroup to a CU");
 constexpr size_t kOwnLds = 128 << 10; // for the staged queries of a workgroup's waves
-constexpr int kCus = 256;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRaise = 8.0f;      // log2: how far a score may pass the reference before sums are rescaled
 
@@ -991,8 +992,24 @@ static int block_of(uint64_t queries, int kv_heads, uint64_t tiles) {
     return queries <= 16 || (queries + 15) / 16 * kv_heads * tiles <= kFewTiles ? 16 : kManyQueries;
 }
 
+// The workspace's parts; its bytes.
+static size_t lay_out(Cut& c, size_t runs, size_t prefix_rows, size_t own_rows, int head_dim, void* workspace) {
+    char* at = (char*)workspace;
+    auto take = [&](size_t n) {
+        char* p = at;
+        at += (n + 255) / 256 * 256;
+        return p;
+    };
+    c.runs = (Run*)take(runs * sizeof(Run));
+    c.prefix_stats = (float2*)take(prefix_rows * sizeof(float2));
+    c.own_stats = (float2*)take(own_rows * sizeof(float2));
+    c.prefix_o = (float*)take(prefix_rows * head_dim * sizeof(float));
+    c.own_o = (float*)take(own_rows * head_dim * sizeof(float));
+    return (size_t)(at - (char*)workspace);
+}
+
 static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int tile, uint32_t prefix_tokens,
-                  uint64_t row_tokens, size_t query_bytes, void* workspace, size_t* bytes) {
+                  uint64_t row_tokens, size_t query_bytes, void* workspace) {
     Cut c{};
     const int group = q_heads / kv_heads;
     c.prefix_tiles = (int)((prefix_tokens + tile - 1) / tile);
@@ -1031,27 +1048,27 @@ static Cut cut_of(uint32_t rows, int q_heads, int kv_heads, int head_dim, int ti
     c.groups = (int)std::min<uint64_t>(most, own_tiles);
     const size_t prefix_rows = (size_t)kv_heads * c.chunks * rows * group;
     const size_t own_rows = ((size_t)c.groups * c.per_group + (size_t)rows * kv_heads) * group;
-    char* at = (char*)workspace;
-    auto take = [&](size_t n) {
-        char* p = at;
-        at += (n + 255) / 256 * 256;
-        return p;
-    };
-    c.runs = (Run*)take((size_t)rows * kv_heads * sizeof(Run));
-    c.prefix_stats = (float2*)take(prefix_rows * sizeof(float2));
-    c.own_stats = (float2*)take(own_rows * sizeof(float2));
-    c.prefix_o = (float*)take(prefix_rows * head_dim * sizeof(float));
-    c.own_o = (float*)take(own_rows * head_dim * sizeof(float));
-    if (bytes) *bytes = (size_t)(at - (char*)workspace);
+    lay_out(c, (size_t)rows * kv_heads, prefix_rows, own_rows, head_dim, workspace);
     return c;
 }
 
+// No call with at most as many rows, tokens a row and prefix tokens takes more: a
+// piece of the prefix goes to a CU, or there is one for each block; a call that
+// takes 16 queries at a time has only such calls below it.
 size_t paged_attn_workspace(uint32_t rows, int q_heads, int kv_heads, int head_dim, int bf16, uint32_t prefix_tokens,
                             uint64_t row_tokens) {
-    size_t bytes = 0;
-    // no call leaves more pieces than one whose queries take the least room
-    cut_of(rows, q_heads, kv_heads, head_dim, bf16 ? 32 : 16, prefix_tokens, row_tokens, 0, nullptr, &bytes);
-    return bytes;
+    const uint64_t tile = bf16 ? 32 : 16, group = q_heads / kv_heads, queries = rows * group;
+    const uint64_t tiles = (prefix_tokens + tile - 1) / tile, all = (uint64_t)kv_heads * tiles * queries;
+    const bool many = tiles && block_of(queries, kv_heads, tiles) == kManyQueries;
+    auto pieces = [&](uint64_t block) {
+        return std::min(all, block * std::max<uint64_t>(kCus, (queries + block - 1) / block * kv_heads));
+    };
+    const uint64_t prefix_rows = std::max(pieces(16), many ? pieces(kManyQueries) : 0);
+    const uint64_t own_tiles = (uint64_t)rows * kv_heads * ((row_tokens + tile - 1) / tile);
+    const uint64_t groups = std::min<uint64_t>(kCus, own_tiles);
+    const uint64_t own_rows = (groups * (many ? kManyWaves : 4) + (uint64_t)rows * kv_heads) * group;
+    Cut c{};
+    return lay_out(c, (size_t)rows * kv_heads, prefix_rows, own_rows, head_dim, nullptr);
 }
 
 // A staged query: 16 bytes for each part, step and quarter.
@@ -1063,7 +1080,7 @@ constexpr size_t query_bytes() {
 template <bool IO, bool KV, int D>
 static hipError_t launch(const PagedAttnArgs& a, hipStream_t st) {
     const Cut c = cut_of(a.rows, a.q_heads, a.pool.kv_heads, D, Form<IO, KV, D>::kTile, a.prefix_tokens,
-                         (uint64_t)a.stride * a.pool.page_tokens.d, query_bytes<IO, KV, D>(), a.workspace, nullptr);
+                         (uint64_t)a.stride * a.pool.page_tokens.d, query_bytes<IO, KV, D>(), a.workspace);
     using F = Form<IO, KV, D>;
     const bool many = c.chunks && c.block == kManyQueries;
     const int waves = many ? kManyWaves : 4;
