@@ -178,7 +178,8 @@ def test_threads_share_a_context(ctx):
 
 
 @pytest.mark.parametrize("rows,vocab,history,biases,dtype", [
-    (96, 4000, 9000, 700, F32), (50, 8191, 16000, 1100, BF16), (1, 1000, 6000, 900, F32)])
+    (96, 4000, 9000, 700, F32), (50, 8191, 16000, 1100, BF16), (1, 1000, 6000, 900, F32), (1100, 4000, 6000, 600, F32),
+    (1100, 4000, 6000, 600, BF16)])
 def test_most_of_a_vocabulary_is_touched(ctx, rows, vocab, history, biases, dtype):
     """More tokens of a slice change than its list holds, more biases than a
     workgroup has threads, many of them for the same tokens."""
@@ -192,6 +193,24 @@ def test_most_of_a_vocabulary_is_touched(ctx, rows, vocab, history, biases, dtyp
     sampling.adjust(ctx, x.cuda(), sampling.rules(**device(u)), out, greedy)
     torch.cuda.synchronize()
     assert same(out.cpu(), want) and np.array_equal(greedy.cpu().numpy().view(np.uint32), ids)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(204, 20480), (205, 20480), (250, 17001), (256, 17001), (257, 17001)])
+def test_slices_that_run_at_once(ctx, dtype, rows, vocab):
+    """1020, 1025, 1250, 1280 and 1285 slices; in place on odd strides."""
+    g = torch.Generator().manual_seed(vocab)
+    u = random_rules(g, rows, vocab, 300, 20, 5)
+    x = torch.randn(rows, vocab, generator=g).to(dtype)
+    want, ids = expect(x, u, vocab)
+    for pad in (0, 3):
+        wide = torch.zeros(rows, vocab + pad, dtype=dtype, device="cuda")
+        wide[:, :vocab] = x.cuda()
+        greedy = torch.empty(rows, dtype=torch.int32, device="cuda")
+        sampling.adjust(ctx, wide[:, :vocab], sampling.rules(**device(u)), greedy=greedy)
+        torch.cuda.synchronize()
+        assert same(wide[:, :vocab].cpu(), want) and np.array_equal(greedy.cpu().numpy().view(np.uint32), ids)
+        assert (wide[:, vocab:] == 0).all()
 
 
 def test_limits_are_refused(ctx):

@@ -13,9 +13,8 @@
 // the biases of one token are summed in their order.
 //
 // The bytes of 32 rows of 151936 take 7.7 us, a copy through this kernel with a
-// mask 11.4; 500 tokens of history make it 16 us and 2500 17: barriers and
-// shared memory between a slice's loads and its stores, and 1216 workgroups
-// where 1024 run at once.  With 64 rows of 9000 tokens 29 us: the histories,
+// mask 11.4; 500 tokens of history make it 14.2 us and 2500 15.7: barriers and
+// shared memory between a slice's loads and its stores.  With 64 rows of 9000 tokens 29 us: the histories,
 // 38 slices of each row reading them from the L2s, are then 88 MB beside the
 // logits' 39.
 #include "zg_paged.hpp"
@@ -285,7 +284,15 @@ static int adjust(const LogitArgs& a, hipStream_t st) {
     // at 32 (2500); slices of 8192, two workgroups to a CU, 19.6 at 32.
     const int slice = a.rows * slices_of(a.vocab, 4096) >= 96 ? 4096 : kLeastSlice, slices = slices_of(a.vocab, slice);
     const dim3 grid(slices, (unsigned)a.rows);
-    if (slice == 4096) logits_adjust_kernel<BF16, WHOLE, 512, 2><<<grid, 512, 0, st>>>(a, slices);
+    // Of 512 threads 1024 workgroups run at once, of 256 the LDS holds 1280: where
+    // that makes one round of two, 32 rows take 15.7 for 17.0 us (2500 tokens of
+    // history; 600: 14.6 for 16.5, 16-bit 12.7 for 15.6; 9000: 19.5 for 20.1).
+    // Elsewhere fewer threads to a history cost as much or more: 34 rows 18.6
+    // for 16.9, 128 rows 49.5 for 46.5, 16 rows with 16000 tokens 19.4 for 15.6.
+    const size_t all = a.rows * slices;
+    if (slice == 4096 && all > 1024 && all <= 1280)
+        logits_adjust_kernel<BF16, WHOLE, 256, 4><<<grid, 256, 0, st>>>(a, slices);
+    else if (slice == 4096) logits_adjust_kernel<BF16, WHOLE, 512, 2><<<grid, 512, 0, st>>>(a, slices);
     else logits_adjust_kernel<BF16, WHOLE, 256, 1><<<grid, 256, 0, st>>>(a, slices);
     return slices;
 }
