@@ -634,10 +634,10 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
  * does not matter.  NaN and infinities among the tokens come through as the
  * formula has them, but that an infinite key or value of a ZG_BF16 cache
  * may make what it enters NaN (the parts of a 32-bit factor can be 0).  A
- * query whose scores are all -inf gets zeros.  |scale| below 2^127.  workspace of zg_paged_attn_workspace_bytes bytes (0 for
- * arguments that the call refuses; as many serve any call with no more rows,
- * tokens a row can hold and prefix tokens), 16-byte aligned, is written and read by
- * the call: calls, and replays of captured ones, that may run at the same
+ * query whose scores are all -inf gets zeros.  |scale| below 2^127.
+ * workspace of zg_paged_attn_workspace_bytes bytes (0 for arguments that the
+ * call refuses; as many serve any call with no more rows, tokens a row can
+ * hold and prefix tokens), 16-byte aligned, is written and read by the call: calls, and replays of captured ones, that may run at the same
  * time need one each.  A captured call keeps prefix_tokens and the pointers,
  * and reads the tables and lengths anew at each replay.  Asynchronous. */
 size_t zg_paged_attn_workspace_bytes(const zg_paged_kv* cache, const zg_paged_rows* rows, size_t q_heads);

@@ -23,10 +23,11 @@ constexpr size_t kMaxStride = (size_t)1 << 32;  // elements: offsets of 2^31 row
 // The context's device for the length of a call; the caller's comes back.
 struct OnDevice {
     int before = -1;
-    bool ok;
+    bool ok = true;
     explicit OnDevice(int device) {
         if (hipGetDevice(&before) != hipSuccess) before = -1;
-        ok = hipSetDevice(device) == hipSuccess;
+        if (before == device) before = -1;  // nothing to bring back
+        else ok = hipSetDevice(device) == hipSuccess;
     }
     ~OnDevice() {
         if (before >= 0) (void)hipSetDevice(before);
