@@ -201,9 +201,7 @@ __global__ __launch_bounds__(T) void logits_adjust_kernel(LogitArgs a, int slice
             } else if (c & kBiased) {
                 v += (double)add[bias_of[i]];
             }
-            float y = (float)v;
-            if constexpr (BF16) y = bf16_to_f32(to_bf16(y));
-            value[i] = __float_as_uint(y);
+            value[i] = BF16 ? (uint32_t)to_bf16(v) << 16 : __float_as_uint((float)v);
         }
         __syncthreads();
     }

@@ -103,6 +103,15 @@ __device__ __forceinline__ uint16_t to_bf16(float x) {
     if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
     return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
 }
+// f64 -> bf16 in one rounding, nearest even: the f32 on the way is rounded to
+// odd (towards zero, its last bit set where anything was dropped), so that its
+// tie is a tie of the 64 bits too.
+__device__ __forceinline__ uint16_t to_bf16(double x) {
+    const float y = (float)x;
+    uint32_t u = __float_as_uint(y);
+    if ((double)y != x) u = (fabs((double)y) > fabs(x) ? u - 1 : u) | 1u;
+    return to_bf16(__uint_as_float(u));
+}
 
 // Four consecutive elements, stored as f32 or bf16.
 template <bool BF16>
