@@ -289,11 +289,18 @@ CONTEXT = []
 
 
 def context():
-    """The program's one context and the stream that its steps run on."""
+    """The program's one context, and the stream that its steps run on: torch's
+    current one.  The library has no handle for torch's default stream, so a
+    program that is still on that one moves to a stream of its own."""
     from zerogravity_amd import _lib as L
     if not CONTEXT:
         CONTEXT.extend([L.Context(0), torch.cuda.Stream()])
-    return CONTEXT
+    stream = torch.cuda.current_stream()
+    if not stream.cuda_stream:
+        CONTEXT[1].wait_stream(stream)
+        torch.cuda.set_stream(CONTEXT[1])
+        stream = CONTEXT[1]
+    return CONTEXT[0], stream
 
 
 def p(t):
@@ -301,12 +308,16 @@ def p(t):
 
 
 def bind(s):
-    """A state's call with its arguments in place, as a decode loop keeps it."""
+    """A state's call with its arguments in place, as a decode loop keeps it,
+    for the stream that is then current."""
     from zerogravity_amd import _lib as L
     from zerogravity_amd import paged, sampling
     case, lib = s["case"], L.lib()
     ctx, stream = context()
     st = stream.cuda_stream
+    for t in s.values():  # made before the program moved, perhaps
+        if isinstance(t, torch.Tensor):
+            t.record_stream(stream)
     if case["op"] == "adjust":
         rules = sampling.rules(history=s["history"], history_lengths=s["history_lengths"], prompt_lengths=s["prompts"],
                                repetition=s["repetition"], frequency=s["frequency"], presence=s["presence"],
