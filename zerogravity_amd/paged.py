@@ -48,12 +48,21 @@ def rows(table, prefix=None, prefix_tokens=0):
     return r
 
 
+def host_ints(a, what):
+    """A host array as int32; what that would cut off or wrap is refused."""
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+        malformed(f"{what}: whole numbers of 32 bits")
+    return np.ascontiguousarray(a, np.int32)
+
+
 def admit(kv, table, lengths, q_heads, prefix=None, prefix_tokens=0):
-    """Whether a batch's page tables, still in host memory (numpy int32), fit
-    the pool; ZgError with the reason if they do not."""
+    """Whether a batch's page tables, still in host memory (numpy int32, or
+    what int32 holds without a change), fit the pool; ZgError with the reason
+    if they do not."""
     import ctypes as C
-    table, lengths = np.ascontiguousarray(table, np.int32), np.ascontiguousarray(lengths, np.int32)
-    shared = None if prefix is None else np.ascontiguousarray(prefix, np.int32)
+    table, lengths = host_ints(table, "page table"), host_ints(lengths, "lengths")
+    shared = None if prefix is None else host_ints(prefix, "prefix pages")
     if table.ndim != 2 or lengths.shape != table.shape[:1]:
         malformed("page table [rows, pages] and lengths [rows]")
     if prefix_tokens > (0 if shared is None else shared.size) * max(1, kv.page_tokens):
