@@ -38,6 +38,13 @@ def on_device(ctx, t, what):
     return t.data_ptr()
 
 
+def written(t, what):
+    """A tensor that a call writes to: autograd does not see that."""
+    import torch
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
+        malformed(f"{what}: written without autograd's knowledge; detach it, or call under torch.no_grad()")
+
+
 def stream_of(ctx, stream):
     """The torch stream of one call: the one given, else the current one."""
     import torch

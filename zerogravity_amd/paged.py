@@ -6,12 +6,13 @@ Thin forms of zg_paged_append_device and zg_paged_attn_device
 two tensors [pages, page_tokens, kv_heads, head_dim], bfloat16 or float32
 (slices of one interleaved pool will do); a row's tokens lie in the pages its
 row of the table lists.  Calls go to torch's current stream, or to the torch
-stream `stream`, and return without waiting.
+stream `stream`, and return without waiting.  No gradient passes through
+them: what they write may not require one.
 """
 import numpy as np
 
 from . import _lib as L
-from ._torch import device_array, dtype_code, launching, malformed, on_device, room, stream_of
+from ._torch import device_array, dtype_code, launching, malformed, on_device, room, stream_of, written
 
 
 def cache(keys, values):
@@ -93,6 +94,8 @@ def append(ctx, kv, r, k, v, positions, q=None, q_out=None, q_norm=None, k_norm=
         if (q.dim() != 3 or q.shape != (tokens, q_heads, kv.head_dim) or q.dtype != k.dtype or q.stride(2) != 1 or
                 q_out is None or q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous()):
             malformed("paged append: q and q_out [tokens, q_heads, head_dim]")
+    for t, name in zip(kv.tensors + (q_out,), ("keys", "values", "q_out")):
+        written(t, name)
     strides = [t.stride(0) if tokens > 1 else t.shape[1] * t.stride(1) for t in (k, v)]
     q_stride = 0 if q is None else q.stride(0) if tokens > 1 else q_heads * q.stride(1)
     args = (device_array(ctx, q_norm, "q_norm", torch.float32, kv.head_dim),
@@ -127,6 +130,7 @@ def attend(ctx, kv, r, lengths, q, scale, out=None, workspace=None, status=None,
     if out is None:
         with torch.cuda.stream(stream_of(ctx, stream)):
             out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    written(out, "out")
     if out.shape != q.shape or out.dtype != q.dtype or out.stride()[1:] != q.stride()[1:]:
         malformed("paged attention: out like q")
     if r.prefix_tokens > (0 if r.tensors[1] is None else r.tensors[1].numel()) * kv.page_tokens:

@@ -3,10 +3,11 @@ grammar's mask, and the highest token left.
 
 A thin form of zg_logits_adjust_device (include/zg_hip.h) over torch tensors
 on the context's device.  Calls go to torch's current stream, or to the torch
-stream `stream`, and return without waiting.
+stream `stream`, and return without waiting.  No gradient passes through
+them: what they write may not require one.
 """
 from . import _lib as L
-from ._torch import device_array, dtype_code, launching, malformed, on_device, room
+from ._torch import device_array, dtype_code, launching, malformed, on_device, room, written
 
 
 def rules(history=None, history_lengths=None, prompt_lengths=None, repetition=None, frequency=None, presence=None,
@@ -52,6 +53,7 @@ def adjust(ctx, logits, u, out=None, greedy=None, record=False, workspace=None, 
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         malformed("logits [rows, vocab]")
     out = logits if out is None else out
+    written(out, "out")
     if out.shape != logits.shape or out.dtype != logits.dtype or (out.shape[1] > 1 and out.stride(1) != 1):
         malformed("out: like logits")
     n, vocab = logits.shape
