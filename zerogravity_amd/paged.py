@@ -82,6 +82,8 @@ def append(ctx, kv, r, k, v, positions, q=None, q_out=None, q_norm=None, k_norm=
     [tokens, q_heads, head_dim], of any token stride; q_out like q,
     contiguous."""
     import torch
+    if k.dim() != 3 or (q is not None and q.dim() != 3):
+        malformed("paged append: q, k and v [tokens, heads, head_dim]")
     tokens = k.shape[0]
     if k.shape[1:] != (kv.kv_heads, kv.head_dim) or v.shape != k.shape or v.dtype != k.dtype:
         malformed("paged append: k and v [tokens, kv_heads, head_dim]")
@@ -91,7 +93,7 @@ def append(ctx, kv, r, k, v, positions, q=None, q_out=None, q_norm=None, k_norm=
     q_heads = 0
     if q is not None:
         q_heads = q.shape[1]
-        if (q.dim() != 3 or q.shape != (tokens, q_heads, kv.head_dim) or q.dtype != k.dtype or q.stride(2) != 1 or
+        if (q.shape != (tokens, q_heads, kv.head_dim) or q.dtype != k.dtype or q.stride(2) != 1 or
                 q_out is None or q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous()):
             malformed("paged append: q and q_out [tokens, q_heads, head_dim]")
     for t, name in zip(kv.tensors + (q_out,), ("keys", "values", "q_out")):
