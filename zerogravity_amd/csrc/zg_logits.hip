@@ -282,13 +282,21 @@ static int adjust(const LogitArgs& a, hipStream_t st) {
     // at 32 (2500); slices of 8192, two workgroups to a CU, 19.6 at 32.
     const int slice = a.rows * slices_of(a.vocab, 4096) >= 96 ? 4096 : kLeastSlice, slices = slices_of(a.vocab, slice);
     const dim3 grid(slices, (unsigned)a.rows);
-    // Of 512 threads 1024 workgroups run at once, of 256 the LDS holds 1280: where
-    // that makes one round of two, 32 rows take 15.7 for 17.0 us (2500 tokens of
-    // history; 600: 14.6 for 16.5, 16-bit 12.7 for 15.6; 9000: 19.5 for 20.1).
-    // Elsewhere fewer threads to a history cost as much or more: 34 rows 18.6
-    // for 16.9, 128 rows 49.5 for 46.5, 16 rows with 16000 tokens 19.4 for 15.6.
-    const size_t all = a.rows * slices;
-    if (slice == 4096 && all > 1024 && all <= 1280)
+    // Of 512 threads 1024 workgroups run at once, of 256 the LDS holds 1280: the
+    // latter are taken where they need fewer rounds, which pays if it halves
+    // them, and of 16-bit logits wherever it spares one; but each thread then
+    // has twice the history, so the longer that may be, the less.  us with 512
+    // and 256 threads, a vocabulary of 151936, 600, 2500, 9000, 16000 tokens of
+    // history: 27 rows (1026 slices) 16.1 15.1, 16.4 16.1, 19.2 19.6, 21.6 23.3;
+    // 32 rows (1216) 18.3 16.4, 18.6 17.6, 21.3 20.9, 24.4 24.7, 16-bit 17.6 14.8,
+    // 17.9 15.5, 20.7 19.4, 23.8 23.3; 64 rows (2432: 3 and 2 rounds) 26.3 25.4,
+    // 26.5 26.7, 30.3 32.9, 16-bit 25.1 23.0, 25.4 24.2, 29.9 30.8; 101 rows (3838:
+    // 4 and 3) 39.8 41.7, 39.4 42.6, 16-bit 33.8 31.7, 34.4 33.2, 41.1 42.2.  In as
+    // many rounds: 34 rows (1292) 18.9 20.5, 16-bit 18.1 18.8; 26 (988) 14.4 15.1.
+    constexpr size_t kMoreHistory = 18432;
+    const size_t all = a.rows * slices, rounds = (all + 1023) / 1024, fewer = (all + 1279) / 1280;
+    const size_t history = a.rules.history ? a.rules.history_stride : 0;
+    if (slice == 4096 && fewer < rounds && (BF16 || fewer == 1) && history * rounds <= kMoreHistory)
         logits_adjust_kernel<BF16, WHOLE, 256, 4><<<grid, 256, 0, st>>>(a, slices);
     else if (slice == 4096) logits_adjust_kernel<BF16, WHOLE, 512, 2><<<grid, 512, 0, st>>>(a, slices);
     else logits_adjust_kernel<BF16, WHOLE, 256, 1><<<grid, 256, 0, st>>>(a, slices);
