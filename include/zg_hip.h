@@ -543,7 +543,11 @@ int zg_gemv_prepared_device(zg_ctx* ctx, const zg_weight* w, size_t m_rows, cons
  * d of head h of slot s of page p is at p * page_stride + (s * kv_heads + h)
  * * head_dim + d of keys and of values, in elements of dtype: a page is a
  * piece of the token-major cache that zg_attn_decode_device takes, and keys
- * and values may be interleaved in one pool.  head_dim 64, 128 or 256; dtype
+ * and values may be interleaved in one pool.  A cache can be copied from one
+ * form to the other, but that entry and the sessions multiply a rotation's
+ * angle up in 32 bits where zg_paged_append_device forms it in 64, so far into
+ * a context the keys of one and the queries of the other part (by up to 2.4e-8
+ * of the position, in radians).  head_dim 64, 128 or 256; dtype
  * ZG_BF16 or ZG_F32; page_tokens 1..65536; page_stride a multiple of 64, at
  * least page_tokens * kv_heads * head_dim; both pointers 16-byte aligned. */
 typedef struct zg_paged_kv {
@@ -587,8 +591,8 @@ int zg_paged_admit(const zg_paged_kv* cache, const zg_paged_rows* rows, const in
  * not), their first `rotate` elements turned in pairs (i, i + rotate/2) by
  * the angle position * theta_scale^i (the pairing of source_rope_kv,
  * lib.rs:1552-1577; the angle is formed in 64 bits and its sine and cosine in
- * 32, where the reference multiplies it up in 32, so the two part by some
- * 1e-6 of the angle), key and value rounded to the cache's type and stored in
+ * 32, where the reference multiplies it up in 32, so the two part by up to
+ * 3e-7 of the angle), key and value rounded to the cache's type and stored in
  * the slot of their position, the query written to q_out.  Replaces the
  * RopeKvRegion (accelerator.rs:205-296) and the cache append for a resident
  * paged cache.  q [tokens] of row stride q_stride with heads q_head_stride
@@ -601,9 +605,9 @@ int zg_paged_admit(const zg_paged_kv* cache, const zg_paged_rows* rows, const in
  * first token, so a row's first own token is at rows->prefix_tokens;
  * negative: the token is skipped, nothing is written for it.
  * token_rows [tokens] (device) is each token's row, NULL: token t belongs to
- * row t.  tokens 1 to 2^24 - 1; rotate 0 to head_dim, a multiple of 8.  The positions of one row in
- * one call differ from each other; which of two tokens at one place stays is
- * not defined.  A row or position outside the table (ZG_STATUS_POSITION) or a
+ * row t.  tokens 1 to 2^24 - 1; rotate 0 to head_dim, a multiple of 8.  The
+ * positions of one row in one call differ from each other; which of two tokens
+ * at one place stays is not defined.  A row or position outside the table (ZG_STATUS_POSITION) or a
  * page outside the pool (ZG_STATUS_PAGE) stores no key and value; the query is
  * written all the same.  To write the prefix itself, give its pages as a row
  * with prefix_tokens 0.  Asynchronous. */
@@ -618,16 +622,20 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
  * prefix's keys and values are read for many rows together.  out[r][h] =
  * sum_t e^(scale q.k_t - m) v_t / sum_t e^(scale q.k_t - m) with kv head h /
  * (q_heads / kv_heads), the softmax of lib.rs:1352-1387 and the value sum of
- * lib.rs:1276-1305 regrouped: sums in 32 bits; 32-bit queries enter the
- * matrix products as three bfloat16 parts (24 bits in all).  No counterpart in
- * the reference, whose cohorts read each row's cache by itself.  q
+ * lib.rs:1276-1305 regrouped: sums in 32 bits.  Over a ZG_BF16 cache 32-bit
+ * queries, and the weights e^(s - m) of 32-bit outputs, enter the matrix
+ * products as three bfloat16 parts, 24 bits in all; the weights of ZG_BF16
+ * outputs as two, which leaves out 2^-16 of each at most and so 2^-16 of sum w
+ * |v| of an output, beside its rounding.  No sigmoid gate is applied.  No
+ * counterpart in the reference, whose cohorts read each row's cache by itself.
+ * q
  * [rows][q_heads * head_dim] of row stride q_stride and out of row stride
  * out_stride, both of dtype ZG_F32 or ZG_BF16, 16-byte aligned, strides
  * multiples of 8; out may be q.  q_heads a multiple of kv_heads, at most 16
  * times it; at most 4096 rows; rows->stride * page_tokens and prefix_tokens
- * at most 2^30, rows * kv_heads * stride * page_tokens below
- * 2^35.  Several tokens of one sequence are rows with the same pages
- * and their own lengths.  A row without any token (length 0, no prefix) gives
+ * at most 2^30, rows * kv_heads * stride * page_tokens below 2^35.  Several
+ * tokens of one sequence are rows with the same pages and their own lengths;
+ * each such row reads them for itself.  A row without any token (length 0, no prefix) gives
  * zeros; a negative length leaves the row's out as it was.  A length past the
  * row's table is cut to it (ZG_STATUS_POSITION); tokens of a page outside the
  * pool are left out (ZG_STATUS_PAGE).  What slots past a row's length hold
@@ -637,8 +645,9 @@ int zg_paged_append_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged
  * query whose scores are all -inf gets zeros.  |scale| below 2^127.
  * workspace of zg_paged_attn_workspace_bytes bytes (0 for arguments that the
  * call refuses; as many serve any call with no more rows, tokens a row can
- * hold and prefix tokens), 16-byte aligned, is written and read by the call: calls, and replays of captured ones, that may run at the same
- * time need one each.  A captured call keeps prefix_tokens and the pointers,
+ * hold and prefix tokens), 16-byte aligned, is written and read by the call:
+ * calls, and replays of captured ones, that may run at the same time need one
+ * each.  A captured call keeps prefix_tokens and the pointers,
  * and reads the tables and lengths anew at each replay.  Asynchronous. */
 size_t zg_paged_attn_workspace_bytes(const zg_paged_kv* cache, const zg_paged_rows* rows, size_t q_heads);
 int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_rows* rows, const int32_t* lengths,
@@ -650,8 +659,8 @@ int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_r
  * prompt first, history_lengths[r] of them (a negative length: the row is
  * left out of the call, its logits and id as they were), the first
  * prompt_lengths[r] (NULL: none) the prompt.  Ids outside the vocabulary
- * count for nothing, nor do the entries past a length, which may be read.  Per row: repetition r > 0 divides a positive and
- * multiplies any other logit of a token in the history; frequency f and
+ * count for nothing, nor do the entries past a length, which may be read.  Per
+ * row: repetition r > 0 divides a positive and multiplies any other logit of a token in the history; frequency f and
  * presence p take f * count + p from a token generated `count` > 0 times
  * (after the prompt).  bias_ids, bias_values [rows][bias_stride],
  * bias_lengths[r] of them: added to their tokens' logits, an id that is there
@@ -680,7 +689,8 @@ typedef struct zg_logit_rules {
 /* Apply the rules to logits [rows][vocab] (row stride ld) of dtype ZG_F32 or
  * ZG_BF16 on the caller's stream and write them to out (row stride out_ld; it
  * may be logits itself, with the same stride): repetition, then frequency
- * and presence, then biases, in 64 bits and rounded once, then the mask.  The
+ * and presence, then biases, in 64 bits and rounded once to dtype, then the
+ * mask.  The
  * readout of zg_greedy over what may be masked: greedy[r] (device, NULL: not
  * asked) is the index of the highest of the row's values as written, the
  * lowest index of equal ones; NaN and -inf are never taken, and 0xffffffff
@@ -690,8 +700,7 @@ typedef struct zg_logit_rules {
  * it needs a history and greedy.  No counterpart in the reference, whose
  * readout is greedy_finite alone (core/src/numerics.rs:124-140).  At most
  * 65535 rows, a vocabulary of 2^30, 65535 biases a row and a history_stride
- * of 2^28.  workspace
- * of zg_logits_adjust_workspace_bytes bytes, 16-byte aligned, needed with
+ * of 2^28.  workspace of zg_logits_adjust_workspace_bytes bytes, 16-byte aligned, needed with
  * greedy (else NULL), one for each call that may run at the same time.
  * Asynchronous. */
 size_t zg_logits_adjust_workspace_bytes(size_t rows, size_t vocab);

@@ -40,7 +40,6 @@ class LogitRules(C.Structure):
                 ("mask_of", P)]
 
 
-
 _SIGS = {
     "zg_version": (C.c_char_p, []),
     "zg_ctx_create": (C.c_int, [C.c_int, C.POINTER(P)]),
