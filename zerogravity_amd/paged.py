@@ -52,7 +52,7 @@ def rows(table, prefix=None, prefix_tokens=0):
 def host_ints(a, what):
     """A host array as int32; what that would cut off or wrap is refused."""
     a = np.asarray(a)
-    if a.size and (a.dtype.kind not in "iu" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+    if a.dtype != np.int32 and a.size and (a.dtype.kind not in "iu" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
         malformed(f"{what}: whole numbers of 32 bits")
     return np.ascontiguousarray(a, np.int32)
 
