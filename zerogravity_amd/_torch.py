@@ -68,13 +68,19 @@ def room(ctx, stream, workspace, need):
 
 
 @contextlib.contextmanager
-def launching(ctx, stream):
-    """The handle of the call's stream.  The library takes a null handle for
-    its context's own stream, which does not wait for torch's default stream;
-    a call on the default stream therefore runs on a stream that waits for it
-    and that it waits for."""
+def launching(ctx, stream, tensors):
+    """The handle of the call's stream.  On another stream than the current
+    one the memory of the call's tensors is kept until it is through, whatever
+    becomes of them.  The library takes a null handle for its context's own
+    stream, which does not wait for torch's default stream; a call on the
+    default stream therefore runs on a stream that waits for it and that it
+    waits for."""
     import torch
     stream = stream_of(ctx, stream)
+    if stream != torch.cuda.current_stream(ctx.device):
+        for t in tensors:
+            if t is not None and t.is_cuda:  # what is not is refused
+                t.record_stream(stream)
     if stream.cuda_stream:
         yield stream.cuda_stream
         return

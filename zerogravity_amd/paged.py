@@ -6,7 +6,8 @@ Thin forms of zg_paged_append_device and zg_paged_attn_device
 two tensors [pages, page_tokens, kv_heads, head_dim], bfloat16 or float32
 (slices of one interleaved pool will do); a row's tokens lie in the pages its
 row of the table lists.  Calls go to torch's current stream, or to the torch
-stream `stream`, and return without waiting.  No gradient passes through
+stream `stream`, and return without waiting; what that stream has to wait for
+before it reads the tensors is the caller's to say.  No gradient passes through
 them: what they write may not require one.
 """
 import numpy as np
@@ -107,7 +108,8 @@ def append(ctx, kv, r, k, v, positions, q=None, q_out=None, q_norm=None, k_norm=
             device_array(ctx, status, "status", torch.int32, 1))
     for t, name in zip(kv.tensors + r.tensors, ("keys", "values", "page table", "prefix pages")):
         on_device(ctx, t, name)
-    with launching(ctx, stream) as st:
+    tensors = kv.tensors + r.tensors + (k, v, positions, q, q_out, q_norm, k_norm, token_rows, status)
+    with launching(ctx, stream, tensors) as st:
         ctx.check(L.lib().zg_paged_append_device(
             ctx.h, kv, r, tokens, q_heads, on_device(ctx, q, "q"), q_stride, 0 if q is None else q.stride(1),
             on_device(ctx, k, "k"), strides[0], on_device(ctx, v, "v"), strides[1], dtype_code(k, "paged append"),
@@ -141,7 +143,8 @@ def attend(ctx, kv, r, lengths, q, scale, out=None, workspace=None, status=None,
     strides = [t.stride(0) if r.rows > 1 else q.shape[1] * kv.head_dim for t in (q, out)]
     for t, name in zip(kv.tensors + r.tensors, ("keys", "values", "page table", "prefix pages")):
         on_device(ctx, t, name)
-    with launching(ctx, stream) as st:
+    tensors = kv.tensors + r.tensors + (lengths, q, workspace, out, status)
+    with launching(ctx, stream, tensors) as st:
         ctx.check(L.lib().zg_paged_attn_device(
             ctx.h, kv, r, device_array(ctx, lengths, "lengths", torch.int32, r.rows), q.shape[1],
             on_device(ctx, q, "q"), strides[0], dtype_code(q, "paged attention"), scale,

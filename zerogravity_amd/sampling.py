@@ -3,7 +3,8 @@ grammar's mask, and the highest token left.
 
 A thin form of zg_logits_adjust_device (include/zg_hip.h) over torch tensors
 on the context's device.  Calls go to torch's current stream, or to the torch
-stream `stream`, and return without waiting.  No gradient passes through
+stream `stream`, and return without waiting; what that stream has to wait for
+before it reads the tensors is the caller's to say.  No gradient passes through
 them: what they write may not require one.
 """
 from . import _lib as L
@@ -64,7 +65,8 @@ def adjust(ctx, logits, u, out=None, greedy=None, record=False, workspace=None, 
     need = L.lib().zg_logits_adjust_workspace_bytes(n, vocab)
     workspace = None if greedy is None else room(ctx, stream, workspace, need)
     strides = [t.stride(0) if n > 1 else vocab for t in (logits, out)]
-    with launching(ctx, stream) as st:
+    tensors = (*u.tensors.values(), logits, out, greedy, workspace, status)
+    with launching(ctx, stream, tensors) as st:
         ctx.check(L.lib().zg_logits_adjust_device(
             ctx.h, n, vocab, on_device(ctx, logits, "logits"), strides[0], dtype_code(logits, "logits"), u,
             on_device(ctx, out, "out"), strides[1], device_array(ctx, greedy, "greedy", torch.int32, n), int(record),
