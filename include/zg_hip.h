@@ -666,9 +666,9 @@ int zg_paged_attn_device(zg_ctx* ctx, const zg_paged_kv* cache, const zg_paged_r
  * bias_lengths[r] of them: added to their tokens' logits, an id that is there
  * twice with the sum.  masks [mask_rows][mask_stride]: bit t % 32 of word t /
  * 32 set allows token t; row r takes mask mask_of[r] (NULL: r), negative: any
- * token is allowed.  A forbidden token's logit becomes -inf, whatever it
- * was.  A rule's arrays are all there or all NULL: the history with its
- * lengths, the biases' three. */
+ * token is allowed, mask_rows or more: none is.  A forbidden token's logit
+ * becomes -inf, whatever it was.  A rule's arrays are all there or all NULL:
+ * the history with its lengths, the biases' three. */
 typedef struct zg_logit_rules {
     int32_t* history;
     size_t history_stride;
